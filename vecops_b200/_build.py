@@ -88,7 +88,10 @@ def build_torch_bridge(force: bool = False, verbose: bool = False) -> Path:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     command = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *includes, str(source),
                "-o", str(TORCH_BRIDGE), f"-L{LIB_DIR}", "-lvecops_b200", "-Wl,-rpath,$ORIGIN",
-               *[f"-L{d}" for d in library_dirs], *[f"-Wl,-rpath,{d}" for d in library_dirs], "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda",
+               *[f"-L{d}" for d in library_dirs], *[f"-Wl,-rpath,{d}" for d in library_dirs],
+               # the C++ runtime torch itself uses, by its file name: a compiler that finds no libstdc++.so link beside it would
+               # put the static one into the bridge, and two runtimes in one process crash when a refusal formats a number
+               "-l:libstdc++.so.6", "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda",
                "-lc10_cuda"]
     subprocess.run(command, check=True, stdout=None if verbose else subprocess.DEVNULL)
     return TORCH_BRIDGE
