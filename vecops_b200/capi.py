@@ -123,6 +123,52 @@ PUSH_KERNEL, PUSH_COPY_ENGINE = 0, 1
 GATHER_MULTICAST = 1
 
 
+# ---- include/vecops_b200/decode_cuda.h
+
+F8_AUTO, F8_GENERIC, F8_STREAM, F8_TILED = range(4)  # VecopsB200MatmulF8Kernel
+
+
+class VecopsB200QuantizeBlocks(Structure):
+    _fields_ = [("struct_size", c_uint32), ("block_rows", c_uint32), ("rows", c_int64), ("cols", c_int64), ("src", c_void_p),
+                ("src_stride_row", c_int64), ("src_stride_col", c_int64), ("src_dtype", c_uint32), ("flags", c_uint32), ("dst", c_void_p),
+                ("dst_stride_row", c_int64), ("scale", c_void_p), ("scale_stride_row", c_int64), ("scale_stride_col", c_int64),
+                ("stream", c_void_p), ("device_index", c_int32), ("reserved", c_uint32)]
+
+
+class VecopsB200MatmulF8(Structure):
+    _fields_ = [("struct_size", c_uint32), ("kernel", c_uint32), ("m", c_int64), ("n", c_int64), ("k", c_int64),
+                ("a", c_void_p), ("a_stride_m", c_int64), ("a_stride_k", c_int64),
+                ("a_scale", c_void_p), ("a_scale_stride_m", c_int64), ("a_scale_stride_k", c_int64),
+                ("b", c_void_p), ("b_stride_n", c_int64), ("b_stride_k", c_int64),
+                ("b_scale", c_void_p), ("b_scale_stride_n", c_int64), ("b_scale_stride_k", c_int64),
+                ("c", c_void_p), ("c_stride_m", c_int64), ("c_stride_n", c_int64), ("c_dtype", c_uint32), ("flags", c_uint32),
+                ("stream", c_void_p), ("device_index", c_int32), ("reserved", c_uint32)]
+
+
+class VecopsB200CacheAppend(Structure):
+    _fields_ = [("struct_size", c_uint32), ("dtype", c_uint32), ("tokens", c_int64), ("q_heads", c_int64), ("kv_heads", c_int64),
+                ("head_dim", c_int64), ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("k", c_void_p),
+                ("k_stride_token", c_int64), ("k_stride_head", c_int64), ("v", c_void_p), ("v_stride_token", c_int64), ("v_stride_head", c_int64),
+                ("q_out", c_void_p), ("q_out_stride_token", c_int64), ("q_out_stride_head", c_int64),
+                ("k_cache", c_void_p), ("k_stride_page", c_int64), ("k_stride_slot", c_int64), ("k_cache_stride_head", c_int64),
+                ("v_cache", c_void_p), ("v_stride_page", c_int64), ("v_stride_slot", c_int64), ("v_cache_stride_head", c_int64),
+                ("pages", c_int64), ("page_size", c_int64), ("slots", c_void_p), ("positions", c_void_p), ("cos_sin", c_void_p),
+                ("cos_sin_stride", c_int64), ("max_positions", c_int64), ("rotary", c_int64), ("interleaved", c_uint32), ("flags", c_uint32),
+                ("stream", c_void_p), ("device_index", c_int32), ("reserved", c_uint32)]
+
+
+class VecopsB200PrefixAttention(Structure):
+    _fields_ = [("struct_size", c_uint32), ("dtype", c_uint32), ("tokens", c_int64), ("batch", c_int64), ("q_heads", c_int64),
+                ("kv_heads", c_int64), ("head_dim", c_int64), ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64),
+                ("out", c_void_p), ("out_stride_token", c_int64), ("out_stride_head", c_int64),
+                ("k_cache", c_void_p), ("k_stride_page", c_int64), ("k_stride_slot", c_int64), ("k_stride_head", c_int64),
+                ("v_cache", c_void_p), ("v_stride_page", c_int64), ("v_stride_slot", c_int64), ("v_stride_head", c_int64),
+                ("pages", c_int64), ("page_size", c_int64), ("prefix_pages", c_void_p), ("prefix_len", c_int64), ("page_table", c_void_p),
+                ("table_stride", c_int64), ("table_width", c_int64), ("lengths", c_void_p), ("query_starts", c_void_p),
+                ("scale", c_float), ("flags", c_uint32), ("workspace", c_void_p), ("workspace_size", c_uint64), ("stream", c_void_p),
+                ("device_index", c_int32), ("reserved", c_uint32)]
+
+
 class VecopsB200DeviceInfo(Structure):
     _fields_ = [("struct_size", c_uint32), ("sm_major", c_int32), ("sm_minor", c_int32), ("sm_count", c_int32),
                 ("l2_bytes", c_uint64), ("hbm_bytes", c_uint64), ("smem_per_block_optin", c_uint64), ("name", c_char * 64)]
@@ -175,6 +221,12 @@ def library() -> ctypes.CDLL:
         lib.vecops_b200_sdpa_workspace.argtypes = [POINTER(VecopsB200Attention), POINTER(c_uint64), e]
         lib.vecops_b200_sdpa_run.argtypes = [POINTER(VecopsB200Attention), e]
         lib.vecops_b200_sdpa_plan.argtypes = [POINTER(VecopsB200Attention), POINTER(c_uint32), POINTER(c_uint32), e]
+        lib.vecops_b200_quantize_blocks.argtypes = [POINTER(VecopsB200QuantizeBlocks), e]
+        lib.vecops_b200_matmul_f8_select.argtypes = [POINTER(VecopsB200MatmulF8), POINTER(c_uint32), e]
+        lib.vecops_b200_matmul_f8_run.argtypes = [POINTER(VecopsB200MatmulF8), e]
+        lib.vecops_b200_cache_append.argtypes = [POINTER(VecopsB200CacheAppend), e]
+        lib.vecops_b200_prefix_sdpa_workspace.argtypes = [POINTER(VecopsB200PrefixAttention), POINTER(c_uint64), e]
+        lib.vecops_b200_prefix_sdpa_run.argtypes = [POINTER(VecopsB200PrefixAttention), e]
         lib.vecops_b200_matmul_allgather_run.argtypes = [POINTER(VecopsB200Matmul), POINTER(VecopsB200Gather), e]
         lib.vecops_b200_kernel_name.argtypes = [c_uint32]
         lib.vecops_b200_kernel_name.restype = c_char_p

@@ -1,4 +1,5 @@
-// Torch bridge: torch.ops.vecops_b200.matmul / matmul_out / sdpa hand CUDA tensors straight to the operator bridge
+// Torch bridge: torch.ops.vecops_b200.matmul / matmul_out / sdpa and the decode-step operators (quantize_blocks,
+// matmul_f8_blocks, cache_append, sdpa_shared_prefix) hand CUDA tensors straight to the operator bridge or the C ABI
 // (vecops_operator_bridge_invoke_v1) on the current stream - dispatcher to C++ to kernel, no Python on the hot path.
 // It stands where vecops' generated Torch adapters stand (python/vecops/ops/torch.py `register` -> generated bridge
 // DSO -> vecops_operator_bridge_invoke_v1, include/vecops/runtime/OperatorBridgeAbi.h:156-158).
@@ -12,8 +13,11 @@
 
 #include <array>
 #include <string>
+#include <tuple>
+#include <utility>
 #include <vector>
 
+#include "vecops_b200/decode_cuda.h"
 #include "vecops_b200/matmul_cuda.h"
 #include "vecops_b200/operator_bridge.h"
 
@@ -191,6 +195,187 @@ at::Tensor sdpa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, d
   return out;
 }
 
+// ---------------------------------------------------------------- the decode step (decode_cuda.h)
+
+void* current_stream(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+// `t` is a CUDA tensor on the device of `like`, of the given rank and type.
+void check_operand(const at::Tensor& t, const at::Tensor& like, int64_t rank, at::ScalarType type, const char* op, const char* name) {
+  TORCH_CHECK(t.is_cuda(), "vecops_b200.", op, ": ", name, " must be a CUDA tensor (there is no CPU path)");
+  TORCH_CHECK(t.get_device() == like.get_device(), "vecops_b200.", op, ": ", name, " is on another device than the first operand");
+  TORCH_CHECK(t.dim() == rank, "vecops_b200.", op, ": ", name, " must have ", rank, " dimensions, not ", t.dim());
+  TORCH_CHECK(t.scalar_type() == type, "vecops_b200.", op, ": ", name, " must be ", type, ", not ", t.scalar_type());
+}
+
+void check_rows(const at::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, "vecops_b200.", op, ": ", name, " must be contiguous along its last dimension");
+}
+
+// x [M,K] -> (e4m3 [M,K] on a row pitch of a multiple of 16, f32 scales [ceil(M / block_rows), ceil(K / 128)])
+std::tuple<at::Tensor, at::Tensor> quantize_blocks(const at::Tensor& x, int64_t block_rows) {
+  TORCH_CHECK(block_rows == 1 || block_rows == 128, "vecops_b200.quantize_blocks: block_rows is 1 or 128, not ", block_rows);
+  TORCH_CHECK(x.is_cuda(), "vecops_b200.quantize_blocks: CUDA tensors only (there is no CPU path)");
+  TORCH_CHECK(x.dim() == 2, "vecops_b200.quantize_blocks: x is [M,K]");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t m = x.size(0), k = x.size(1), pitch = (k + 15) / 16 * 16;
+  at::Tensor q = at::empty({m, pitch}, x.options().dtype(at::kFloat8_e4m3fn));
+  if (pitch != k) q = q.narrow(1, 0, k);
+  at::Tensor scale = at::empty({(m + block_rows - 1) / block_rows, (k + 127) / 128}, x.options().dtype(at::kFloat));
+  VecopsB200QuantizeBlocks r{};
+  r.struct_size = sizeof(r);
+  r.block_rows = static_cast<uint32_t>(block_rows);
+  r.rows = m, r.cols = k;
+  r.src = x.data_ptr(), r.src_stride_row = x.stride(0), r.src_stride_col = x.stride(1);
+  r.src_dtype = dtype_code(x.scalar_type());
+  r.flags = VECOPS_B200_MATMUL_FLAG_ASYNC;
+  r.dst = q.data_ptr(), r.dst_stride_row = pitch;
+  r.scale = scale.data_ptr<float>(), r.scale_stride_row = scale.stride(0), r.scale_stride_col = scale.stride(1);
+  r.stream = current_stream(x);
+  r.device_index = static_cast<int32_t>(x.get_device());
+  ErrorText error;
+  error.check(vecops_b200_quantize_blocks(&r, &error.record), "quantize_blocks");
+  return {q, scale};
+}
+
+// C[M,N] = sum over 128-blocks of K of a_scale * b_scale * (A_block . B_block^T)
+at::Tensor matmul_f8_blocks(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b_nk, const at::Tensor& b_scale,
+                            c10::optional<at::ScalarType> out_dtype) {
+  constexpr const char* op = "matmul_f8_blocks";
+  check_operand(a, a, 2, at::kFloat8_e4m3fn, op, "a");
+  check_operand(b_nk, a, 2, at::kFloat8_e4m3fn, op, "b_nk");
+  check_operand(a_scale, a, 2, at::kFloat, op, "a_scale");
+  check_operand(b_scale, a, 2, at::kFloat, op, "b_scale");
+  const int64_t m = a.size(0), k = a.size(1), n = b_nk.size(0), blocks = (k + 127) / 128;
+  TORCH_CHECK(b_nk.size(1) == k, "vecops_b200.matmul_f8_blocks: a is [M,", k, "], b_nk [N,", b_nk.size(1), "]");
+  TORCH_CHECK(a_scale.size(0) == m && a_scale.size(1) == blocks, "vecops_b200.matmul_f8_blocks: a_scale must be [", m, ",", blocks, "]");
+  TORCH_CHECK(b_scale.size(0) == (n + 127) / 128 && b_scale.size(1) == blocks, "vecops_b200.matmul_f8_blocks: b_scale must be [", (n + 127) / 128, ",",
+              blocks, "]");
+  const c10::cuda::CUDAGuard guard(a.device());
+  at::Tensor c = at::empty({m, n}, a.options().dtype(out_dtype.has_value() ? *out_dtype : at::kBFloat16));
+  VecopsB200MatmulF8 r{};
+  r.struct_size = sizeof(r);
+  r.m = m, r.n = n, r.k = k;
+  r.a = a.data_ptr(), r.a_stride_m = a.stride(0), r.a_stride_k = a.stride(1);
+  r.b = b_nk.data_ptr(), r.b_stride_n = b_nk.stride(0), r.b_stride_k = b_nk.stride(1);
+  r.a_scale = a_scale.data_ptr<float>(), r.a_scale_stride_m = a_scale.stride(0), r.a_scale_stride_k = a_scale.stride(1);
+  r.b_scale = b_scale.data_ptr<float>(), r.b_scale_stride_n = b_scale.stride(0), r.b_scale_stride_k = b_scale.stride(1);
+  r.c = c.data_ptr(), r.c_stride_m = c.stride(0), r.c_stride_n = c.stride(1);
+  r.c_dtype = dtype_code(c.scalar_type());
+  r.flags = VECOPS_B200_MATMUL_FLAG_ASYNC;
+  r.stream = current_stream(a);
+  r.device_index = static_cast<int32_t>(a.get_device());
+  ErrorText error;
+  error.check(vecops_b200_matmul_f8_run(&r, &error.record), "matmul_f8_blocks");
+  return c;
+}
+
+// q [T,Hq,D], k and v [T,Hkv,D] into k_cache, v_cache [pages,page_size,Hkv,D] at slots [T]; returns the rotated q
+at::Tensor cache_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor k_cache, at::Tensor v_cache, const at::Tensor& slots,
+                        const at::Tensor& positions, const at::Tensor& cos_sin, bool interleaved) {
+  constexpr const char* op = "cache_append";
+  check_operand(q, q, 3, q.scalar_type(), op, "q");
+  check_operand(k, q, 3, q.scalar_type(), op, "k");
+  check_operand(v, q, 3, q.scalar_type(), op, "v");
+  check_operand(k_cache, q, 4, q.scalar_type(), op, "k_cache");
+  check_operand(v_cache, q, 4, q.scalar_type(), op, "v_cache");
+  check_operand(slots, q, 1, at::kLong, op, "slots");
+  check_operand(positions, q, 1, at::kLong, op, "positions");
+  check_operand(cos_sin, q, 2, at::kFloat, op, "cos_sin");
+  const int64_t t = q.size(0), d = q.size(2), hkv = k.size(1);
+  TORCH_CHECK(k.size(0) == t && k.size(2) == d && v.sizes() == k.sizes(), "vecops_b200.cache_append: q is [T,Hq,D], k and v are [T,Hkv,D]");
+  TORCH_CHECK(k_cache.size(2) == hkv && k_cache.size(3) == d && v_cache.sizes() == k_cache.sizes(),
+              "vecops_b200.cache_append: k_cache and v_cache are [pages,page_size,", hkv, ",", d, "]");
+  TORCH_CHECK(slots.size(0) == t && positions.size(0) == t, "vecops_b200.cache_append: slots and positions are [T]");
+  TORCH_CHECK(slots.is_contiguous() && positions.is_contiguous(), "vecops_b200.cache_append: slots and positions must be contiguous");
+  TORCH_CHECK(cos_sin.size(1) <= d && cos_sin.size(1) % 2 == 0, "vecops_b200.cache_append: cos_sin is [positions,R] with R even and at most ", d);
+  for (const auto& [tensor, name] : {std::pair<const at::Tensor&, const char*>{q, "q"}, {k, "k"}, {v, "v"}, {k_cache, "k_cache"}, {v_cache, "v_cache"},
+                                     {cos_sin, "cos_sin"}})
+    check_rows(tensor, op, name);
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor q_out = at::empty(q.sizes(), q.options());
+  VecopsB200CacheAppend r{};
+  r.struct_size = sizeof(r);
+  r.dtype = dtype_code(q.scalar_type());
+  r.tokens = t, r.q_heads = q.size(1), r.kv_heads = hkv, r.head_dim = d;
+  r.q = q.data_ptr(), r.q_stride_token = q.stride(0), r.q_stride_head = q.stride(1);
+  r.k = k.data_ptr(), r.k_stride_token = k.stride(0), r.k_stride_head = k.stride(1);
+  r.v = v.data_ptr(), r.v_stride_token = v.stride(0), r.v_stride_head = v.stride(1);
+  r.q_out = q_out.data_ptr(), r.q_out_stride_token = q_out.stride(0), r.q_out_stride_head = q_out.stride(1);
+  r.k_cache = k_cache.data_ptr(), r.k_stride_page = k_cache.stride(0), r.k_stride_slot = k_cache.stride(1), r.k_cache_stride_head = k_cache.stride(2);
+  r.v_cache = v_cache.data_ptr(), r.v_stride_page = v_cache.stride(0), r.v_stride_slot = v_cache.stride(1), r.v_cache_stride_head = v_cache.stride(2);
+  r.pages = k_cache.size(0), r.page_size = k_cache.size(1);
+  r.slots = slots.data_ptr<int64_t>(), r.positions = positions.data_ptr<int64_t>();
+  r.cos_sin = cos_sin.data_ptr<float>(), r.cos_sin_stride = cos_sin.stride(0);
+  r.max_positions = cos_sin.size(0), r.rotary = cos_sin.size(1);
+  r.interleaved = interleaved ? 1 : 0;
+  r.flags = VECOPS_B200_MATMUL_FLAG_ASYNC;
+  r.stream = current_stream(q);
+  r.device_index = static_cast<int32_t>(q.get_device());
+  ErrorText error;
+  error.check(vecops_b200_cache_append(&r, &error.record), "cache_append");
+  return q_out;
+}
+
+// q [T,Hq,D] against the shared prefix and each sequence's own suffix in k_cache, v_cache [pages,page_size,Hkv,D]
+at::Tensor sdpa_shared_prefix(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& prefix_pages, int64_t prefix_len,
+                              const at::Tensor& page_table, const at::Tensor& lengths, double scale, const c10::optional<at::Tensor>& query_starts) {
+  constexpr const char* op = "sdpa_shared_prefix";
+  check_operand(q, q, 3, q.scalar_type(), op, "q");
+  check_operand(k_cache, q, 4, q.scalar_type(), op, "k_cache");
+  check_operand(v_cache, q, 4, q.scalar_type(), op, "v_cache");
+  check_operand(prefix_pages, q, 1, at::kInt, op, "prefix_pages");
+  check_operand(page_table, q, 2, at::kInt, op, "page_table");
+  check_operand(lengths, q, 1, at::kInt, op, "lengths");
+  const int64_t t = q.size(0), hq = q.size(1), d = q.size(2), hkv = k_cache.size(2), batch = page_table.size(0);
+  TORCH_CHECK(k_cache.size(3) == d && v_cache.sizes() == k_cache.sizes(), "vecops_b200.sdpa_shared_prefix: k_cache and v_cache are [pages,page_size,Hkv,", d, "]");
+  TORCH_CHECK(hkv > 0 && hq % hkv == 0, "vecops_b200.sdpa_shared_prefix: ", hq, " query heads over ", hkv, " key heads");
+  TORCH_CHECK(prefix_len >= 0 && k_cache.size(1) > 0 && (prefix_len + k_cache.size(1) - 1) / k_cache.size(1) <= prefix_pages.size(0),
+              "vecops_b200.sdpa_shared_prefix: prefix_pages is too short for ", prefix_len, " keys in pages of ", k_cache.size(1));
+  TORCH_CHECK(lengths.size(0) == batch, "vecops_b200.sdpa_shared_prefix: lengths is [", batch, "]");
+  TORCH_CHECK(prefix_pages.is_contiguous() && lengths.is_contiguous(), "vecops_b200.sdpa_shared_prefix: prefix_pages and lengths must be contiguous");
+  const bool ragged = query_starts.has_value() && query_starts->defined();
+  if (ragged) {
+    check_operand(*query_starts, q, 1, at::kInt, op, "query_starts");
+    TORCH_CHECK(query_starts->size(0) == batch + 1 && query_starts->is_contiguous(), "vecops_b200.sdpa_shared_prefix: query_starts is a contiguous [", batch + 1, "]");
+  } else {
+    TORCH_CHECK(t == batch, "vecops_b200.sdpa_shared_prefix: without query_starts every sequence has one token (", t, " tokens, ", batch, " sequences)");
+  }
+  check_rows(q, op, "q");
+  check_rows(k_cache, op, "k_cache");
+  check_rows(v_cache, op, "v_cache");
+  check_rows(page_table, op, "page_table");
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  VecopsB200PrefixAttention r{};
+  r.struct_size = sizeof(r);
+  r.dtype = dtype_code(q.scalar_type());
+  r.tokens = t, r.batch = batch, r.q_heads = hq, r.kv_heads = hkv, r.head_dim = d;
+  r.q = q.data_ptr(), r.q_stride_token = q.stride(0), r.q_stride_head = q.stride(1);
+  r.out = out.data_ptr(), r.out_stride_token = out.stride(0), r.out_stride_head = out.stride(1);
+  r.k_cache = k_cache.data_ptr(), r.k_stride_page = k_cache.stride(0), r.k_stride_slot = k_cache.stride(1), r.k_stride_head = k_cache.stride(2);
+  r.v_cache = v_cache.data_ptr(), r.v_stride_page = v_cache.stride(0), r.v_stride_slot = v_cache.stride(1), r.v_stride_head = v_cache.stride(2);
+  r.pages = k_cache.size(0), r.page_size = k_cache.size(1);
+  r.prefix_pages = prefix_pages.data_ptr<int32_t>(), r.prefix_len = prefix_len;
+  r.page_table = page_table.data_ptr<int32_t>(), r.table_stride = page_table.stride(0), r.table_width = page_table.size(1);
+  r.lengths = lengths.data_ptr<int32_t>();
+  r.query_starts = ragged ? query_starts->data_ptr<int32_t>() : nullptr;
+  r.scale = static_cast<float>(scale);
+  r.flags = VECOPS_B200_MATMUL_FLAG_ASYNC;
+  r.stream = current_stream(q);
+  r.device_index = static_cast<int32_t>(q.get_device());
+  ErrorText error;
+  uint64_t need = 0;
+  error.check(vecops_b200_prefix_sdpa_workspace(&r, &need, &error.record), "sdpa_shared_prefix workspace query");
+  at::Tensor scratch;
+  if (need != 0) {  // (torch's allocator hands out blocks on 512-byte boundaries)
+    scratch = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
+    r.workspace = scratch.data_ptr();
+    r.workspace_size = need;
+  }
+  error.check(vecops_b200_prefix_sdpa_run(&r, &error.record), "sdpa_shared_prefix");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(vecops_b200, m) {
@@ -199,10 +384,20 @@ TORCH_LIBRARY(vecops_b200, m) {
   m.def("matmul_out(Tensor a, Tensor b_nk, Tensor(a!) c, Tensor? column_scale=None, Tensor? cin=None, float alpha=1.0, int activation=0, "
         "float clamp_lo=0.0, float clamp_hi=0.0, Tensor? row_scale=None) -> ()");
   m.def("sdpa(Tensor q, Tensor k, Tensor v, float scale, int causal=0, Tensor? key_mask=None, Tensor? bias=None, ScalarType? out_dtype=None) -> Tensor");
+  m.def("quantize_blocks(Tensor x, int block_rows=1) -> (Tensor, Tensor)");
+  m.def("matmul_f8_blocks(Tensor a, Tensor a_scale, Tensor b_nk, Tensor b_scale, ScalarType? out_dtype=None) -> Tensor");
+  m.def("cache_append(Tensor q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, Tensor positions, Tensor cos_sin, "
+        "bool interleaved=False) -> Tensor");
+  m.def("sdpa_shared_prefix(Tensor q, Tensor k_cache, Tensor v_cache, Tensor prefix_pages, int prefix_len, Tensor page_table, Tensor lengths, "
+        "float scale, Tensor? query_starts=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(vecops_b200, CUDA, m) {
   m.impl("matmul", &matmul);
   m.impl("matmul_out", &matmul_out);
   m.impl("sdpa", &sdpa);
+  m.impl("quantize_blocks", &quantize_blocks);
+  m.impl("matmul_f8_blocks", &matmul_f8_blocks);
+  m.impl("cache_append", &cache_append);
+  m.impl("sdpa_shared_prefix", &sdpa_shared_prefix);
 }
