@@ -149,11 +149,20 @@ __device__ __forceinline__ void cluster_sync_all() {
                "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The two halves of the same barrier, for work that fits between them.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // Read one float from another CTA's shared memory (`cluster_addr` from map_to_cta).
 __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
   float value;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(value) : "r"(cluster_addr) : "memory");
   return value;
+}
+
+// Write one float into another CTA's shared memory (`cluster_addr` from map_to_cta).
+__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float value) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(value) : "memory");
 }
 
 // Arrive on a barrier that may live in the peer CTA (`cluster_addr` from map_to_cta).
@@ -349,6 +358,29 @@ __device__ __forceinline__ void umma_tf32(uint32_t tmem_d, uint64_t a_desc, uint
       : "memory");
 }
 
+// kind::f8f6f4: one byte per element in shared memory whatever the format; K = 32 per instruction (32 bytes of a K-major row).
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Pair forms: issued by one thread of the leader CTA; A is 256 rows (128 per CTA), B is N rows (N/2 per CTA), each CTA
 // reading its own shared memory at the descriptor's address and accumulating its 128 rows of D in its own TMEM.
 __device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -402,6 +434,17 @@ __device__ __forceinline__ void tmem_load_32x32(uint32_t taddr, uint32_t (&v)[32
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
         "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
         "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_load_32x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr)
       : "memory");
 }
@@ -470,6 +513,7 @@ enum : uint32_t {
   kUmmaF16 = 0,
   kUmmaBF16 = 1,
   kUmmaTF32 = 2,
+  kUmmaE4M3 = 0,
   kUmmaU8 = 0,
   kUmmaS8 = 1,
   kUmmaAccF16 = 0,
