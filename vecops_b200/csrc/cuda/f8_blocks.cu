@@ -166,7 +166,7 @@ int32_t run_tiled(const VecopsB200MatmulF8& q, const DecodeDevice& device, Vecop
   if (tma_store) {
     const uint64_t dims[2] = {static_cast<uint64_t>(q.n), static_cast<uint64_t>(q.m)};
     const uint64_t strides[1] = {static_cast<uint64_t>(q.c_stride_m * kElem)};
-    const uint32_t box[2] = {static_cast<uint32_t>(128 / kElem), 32};
+    const uint32_t box[2] = {static_cast<uint32_t>(128 / kElem), G::kOutRows};
     const CUtensorMapDataType type = q.c_dtype == VECOPS_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : q.c_dtype == VECOPS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     rc = shim_encode_map(&map_c, type, 2, q.c, dims, strides, box, error);

@@ -60,6 +60,13 @@ struct F8StreamArgs {
   uint32_t* status;
 };
 
+// A scale, fetched where the source says: an ordinary load may be moved down to its first use, behind the waits it is meant to overlap.
+__device__ __forceinline__ float f8_load_scale(const float* p) {
+  float x;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(x) : "l"(p));
+  return x;
+}
+
 template <int kColsT, typename OutT>
 __global__ void __launch_bounds__(F8Stream<kColsT>::kThreads, F8Stream<kColsT>::kCtasPerSm)
 f8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const F8StreamArgs p, int slices) {
@@ -162,11 +169,22 @@ f8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       const int i = kb - kb_begin, acc = i & 1;
       if (i % G::kScaleBlocks == 0) {
         if (i != 0) asm volatile("bar.sync 1, %0;" ::"n"(G::kPromoteWarps * 32) : "memory");  // the previous scales have been used
-        for (int e = thread; e < G::kScaleBlocks * G::kCols; e += G::kPromoteWarps * 32) {
-          const int block = e % G::kScaleBlocks, row = e / G::kScaleBlocks;
-          float s = 0.f;
-          if (row < p.m && kb + block < kb_end) s = p.a_scale[row * p.as_sm + (kb + block) * p.as_sk] * b_scale[(kb + block) * p.bs_sk];
-          scales[block * G::kCols + row] = s;
+        // a thread's scales belong to one block: one weight scale, and the loads of all its rows in flight together
+        constexpr int kRowStep = G::kPromoteWarps * 32 / G::kScaleBlocks, kRows = G::kCols / kRowStep;
+        const int block = thread % G::kScaleBlocks, first_row = thread / G::kScaleBlocks;
+        const bool there = kb + block < kb_end;
+        const float bs = there ? f8_load_scale(b_scale + (kb + block) * p.bs_sk) : 0.f;
+        constexpr int kTogether = kRows < 16 ? kRows : 16;
+#pragma unroll 1
+        for (int r0 = 0; r0 < kRows && r0 * kRowStep < p.m; r0 += kTogether) {
+          float s[kTogether];
+#pragma unroll
+          for (int r = 0; r < kTogether; ++r) {
+            const int row = first_row + (r0 + r) * kRowStep;
+            s[r] = there && row < p.m ? f8_load_scale(p.a_scale + row * p.as_sm + (kb + block) * p.as_sk) : 0.f;
+          }
+#pragma unroll
+          for (int r = 0; r < kTogether; ++r) scales[block * G::kCols + first_row + (r0 + r) * kRowStep] = s[r] * bs;
         }
         asm volatile("bar.sync 1, %0;" ::"n"(G::kPromoteWarps * 32) : "memory");
       }

@@ -2,15 +2,19 @@
 //
 //     C[m,n] = sum_b (sa[m,b] sb[n/128,b]) sum_{k in b} A[m,k] B[n,k]
 //
-// A block's scales apply to its sum over 128 k, so each 128-k step of the main loop is an accumulation of its own: four
-// tcgen05.mma.cta_group::2 of 32 k into one of two 256-column fp32 accumulators in tensor memory, which eight warps then
-// read back and add, scaled, to totals in registers - 128 a thread - while the tensor cores fill the other one.  A thread
-// owns one row of C and 128 columns of it, all of one weight block: one factor sa * sb per step, one fused multiply-add
-// per element (two per instruction, fma.rn.f32x2).  Roles, per CTA:
+// A block's scales apply to its sum over 128 k, so every 128-k step of the main loop is an accumulation of its own, which
+// eight warps read back from tensor memory and add, scaled, to totals in registers while the tensor cores work on the next.
+// What bounds the kernel is the round trip MMA -> commit -> read-back -> arrival -> MMA of one accumulator, so tensor
+// memory is cut into four accumulators of 128 columns (two per step) rather than two of 256: three are in flight while
+// one is read.  Roles, per CTA:
 //   warp 0      TMA: its 128 rows of A and its 128 of the tile's 256 rows of B per step, a ring of kStages
-//   warp 1      (leader CTA) issues the MMAs of the pair
-//   warps 2-9   totals, then the store of the tile through shared memory by TMA (or directly where C cannot take that)
-// Persistent: pairs walk the tiles `worker, worker + workers, ...`; the MMAs of the next tile start while this one is stored.
+//   warp 1      (leader CTA) issues tcgen05.mma.cta_group::2, M = 256, N = 128, four of 32 k per accumulator
+//   warps 2-3   fetch the scales into a ring in shared memory, up to 32 steps ahead (fetched by the totals' own threads, 32
+//               rows a warp and each in a line of its own, they took as long as the product itself)
+//   warps 4-11  totals - a thread owns one row and 128 columns of C, all of one weight block: one factor sa * sb per step
+//               and one fused multiply-add per element, two per instruction - then the store of the tile by TMA
+// Of a pair MMA with N = 128 each CTA feeds 64 rows of B: accumulator s of a step holds the tile's columns [64 s, 64 s + 64)
+// and [128 + 64 s, 128 + 64 s + 64).  Persistent: pairs walk the tiles `worker, worker + workers, ...`.
 #pragma once
 
 #include "f8_stream.cuh"
@@ -22,16 +26,27 @@ struct F8Tiled {
   static constexpr int kOperandBytes = 128 * 128;  // 128 rows x 128 bytes of A, and as much of B
   static constexpr int kStageBytes = 2 * kOperandBytes;
   static constexpr int kStages = 6;
+  static constexpr int kAccumulators = 4, kAccColumns = 128;
   static constexpr int kTotalWarps = 8;
-  static constexpr int kThreads = 32 * (2 + kTotalWarps);
-  static constexpr int kStageOutBytes = 32 * 128;  // 32 rows x 128 bytes of C, per warp
+  static constexpr int kFirstTotalWarp = 4;  // register shares are per warpgroup
+  static constexpr int kThreads = 32 * (kFirstTotalWarp + kTotalWarps);
+  // 384 threads x 168 registers at launch; the totals take what the other warpgroup gives up: (56 + 2 x 224) x 128 = 168 x 384
+  static constexpr int kFewRegisters = 56, kManyRegisters = 224;
+  static constexpr int kOutRows = 16;                        // rows of C a warp stages at a time, 128 bytes of each
   static constexpr int kOutOffset = kStages * kStageBytes;
-  static constexpr int kBarrierOffset = kOutOffset + kTotalWarps * kStageOutBytes;
-  static constexpr int kSmemBytes = kBarrierOffset + 256 + 1024;
+  static constexpr int kOutBytes = kTotalWarps * kOutRows * 128;
+  static constexpr int kScaleSteps = 4, kScaleSlots = 8;     // a slot holds four steps' scales of the tile's 128 rows and two weight blocks
+  static constexpr int kScaleOffset = kOutOffset + kOutBytes;
+  static constexpr int kSlotFloats = kScaleSteps * (128 + 2);
+  static constexpr int kBarrierOffset = kScaleOffset + kScaleSlots * kSlotFloats * 4;
+  static constexpr int kBarriers = 3 * kStages + kAccumulators + 2 * kScaleSlots;
+  static constexpr int kSmemBytes = kBarrierOffset + kBarriers * 8 + 8 + 1024;
   static constexpr int kTmemColumns = 512;
   static constexpr long long kGroupBytes = 32ll << 20;  // raster: row tiles holding this much of A share each sweep over N
 };
+static_assert((F8Tiled::kFewRegisters + 2 * F8Tiled::kManyRegisters) * 128 <= 168 * F8Tiled::kThreads, "register split");
 static_assert(F8Tiled::kSmemBytes <= 227 * 1024, "shared memory budget");
+static_assert(F8Tiled::kBarrierOffset % 8 == 0, "barriers are 8-byte words");
 
 // acc += v * s on two floats at once
 __device__ __forceinline__ void f8_fma2(float2& acc, uint32_t v0, uint32_t v1, float s) {
@@ -51,12 +66,15 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-  const uint32_t full_bar = smem_base + G::kBarrierOffset;      // [stages] both CTAs' tiles landed   (TMA -> MMA; the leader's)
-  const uint32_t empty_bar = full_bar + 8 * G::kStages;         // [stages] tiles multiplied          (MMA -> TMA of both)
-  const uint32_t tmem_full_bar = empty_bar + 8 * G::kStages;    // [2] a step's sums are ready        (MMA -> totals of both)
-  const uint32_t tmem_empty_bar = tmem_full_bar + 16;           // [2] ... and have been read         (totals of both -> MMA; the leader's)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + G::kBarrierOffset + 16 * G::kStages + 32);
+  const uint32_t full_bar = smem_base + G::kBarrierOffset;        // [stages] both CTAs' tiles landed          (TMA -> MMA; the leader's)
+  const uint32_t done_bar = full_bar + 8 * G::kStages;            // [stages][2] accumulator s of the step ready (MMA -> totals of both;
+                                                                  //             s = 1: the stage is free, too -> TMA of both)
+  const uint32_t read_bar = done_bar + 16 * G::kStages;           // [accumulators] it has been read           (totals of both -> MMA; the leader's)
+  const uint32_t scale_full_bar = read_bar + 8 * G::kAccumulators;  // [slots]
+  const uint32_t scale_empty_bar = scale_full_bar + 8 * G::kScaleSlots;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + G::kBarrierOffset + 8 * G::kBarriers);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  float* scale_ring = reinterpret_cast<float*>(smem_gen + G::kScaleOffset);  // [slot][step][128 rows of A, 2 blocks of B]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_cta_rank();
@@ -68,11 +86,13 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kStages; ++s) {
       mbar_init(full_bar + 8 * s, 1);
-      mbar_init(empty_bar + 8 * s, 1);
+      mbar_init(done_bar + 16 * s, 1);
+      mbar_init(done_bar + 16 * s + 8, 1);
     }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(tmem_full_bar + 8 * a, 1);
-      mbar_init(tmem_empty_bar + 8 * a, 2 * G::kTotalWarps);
+    for (int a = 0; a < G::kAccumulators; ++a) mbar_init(read_bar + 8 * a, 2 * G::kTotalWarps);
+    for (int s = 0; s < G::kScaleSlots; ++s) {
+      mbar_init(scale_full_bar + 8 * s, 2);
+      mbar_init(scale_empty_bar + 8 * s, G::kTotalWarps);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -97,8 +117,9 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     *abort_flag = 1;
   };
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < G::kFirstTotalWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kFewRegisters));
+    if (warp == 0 && lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -106,7 +127,7 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         int tm, tn;
         tile_coords(tile, tiles_m, tiles_n, raster_group, tm, tn);
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1u, abort_flag)) {
+          if (!mbar_wait(done_bar + 16 * stage + 8, phase ^ 1u, abort_flag)) {
             give_up(kStatusProducerWait);
             ok = false;
             break;
@@ -119,123 +140,173 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           if (++stage == G::kStages) stage = 0, phase ^= 1u;
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = umma_instr_desc(kUmmaAccF32, kUmmaE4M3, kUmmaE4M3, 256, 256);
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = umma_instr_desc(kUmmaAccF32, kUmmaE4M3, kUmmaE4M3, 256, G::kAccColumns);
+      int stage = 0, pair = 0;  // pair: accumulators 2 * pair and 2 * pair + 1
+      uint32_t phase = 0, pair_phase = 0;
       bool ok = true;
       for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait_cluster(tmem_empty_bar + 8 * acc, acc_phase ^ 1u, abort_flag)) {
-            give_up(kStatusMmaWaitTmem);
-            ok = false;
-            break;
-          }
+        for (int kb = 0; ok && kb < num_kb; ++kb) {
           if (!mbar_wait(full_bar + 8 * stage, phase, abort_flag)) {
             give_up(kStatusMmaWaitFull);
             ok = false;
             break;
           }
-          tcgen05_fence_after_sync();
           const uint64_t a_desc = umma_smem_desc_sw128(smem_base + stage * G::kStageBytes);
           const uint64_t b_desc = umma_smem_desc_sw128(smem_base + stage * G::kStageBytes + G::kOperandBytes);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) umma_f8_pair(tmem_base + acc * G::kTile, a_desc + 2 * kk, b_desc + 2 * kk, idesc, kk != 0 ? 1u : 0u);
-          umma_commit_pair(empty_bar + 8 * stage);
-          umma_commit_pair(tmem_full_bar + 8 * acc);
+          for (int sub = 0; sub < 2; ++sub) {
+            if (!mbar_wait(read_bar + 8 * (2 * pair + sub), pair_phase ^ 1u, abort_flag)) {
+              give_up(kStatusMmaWaitTmem);
+              ok = false;
+              break;
+            }
+            tcgen05_fence_after_sync();
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f8_pair(tmem_base + (2 * pair + sub) * G::kAccColumns, a_desc + 2 * kk, b_desc + sub * (64 * 128 >> 4) + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+            umma_commit_pair(done_bar + 16 * stage + 8 * sub);
+          }
           if (++stage == G::kStages) stage = 0, phase ^= 1u;
-          acc ^= 1;
-          if (acc == 0) acc_phase ^= 1u;
+          pair ^= 1;
+          if (pair == 0) pair_phase ^= 1u;
+        }
+      }
+    } else if (warp >= 2) {
+      const int row_in_tile = (warp - 2) * 64 + 2 * lane;  // two rows a thread
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = worker; ok && tile < num_tiles; tile += workers) {
+        int tm, tn;
+        tile_coords(tile, tiles_m, tiles_n, raster_group, tm, tn);
+        const int row = tm * G::kTile + static_cast<int>(rank) * 128 + row_in_tile;
+        const int block = 2 * tn + (warp - 2);  // weight block fetched by lanes 0..3 of the warp, one step each
+        const float* a_scale = p.a_scale + static_cast<long long>(row) * p.as_sm;
+        const float* b_scale = p.b_scale + static_cast<long long>(block) * p.bs_sn;
+        for (int kb = 0; kb < num_kb; kb += G::kScaleSteps) {
+          float a[G::kScaleSteps][2], b = 0.f;
+#pragma unroll
+          for (int g = 0; g < G::kScaleSteps; ++g) {  // (what lies past the matrix is never stored: its factor is 0)
+            a[g][0] = kb + g < num_kb && row < p.m ? __ldg(a_scale + (kb + g) * p.as_sk) : 0.f;
+            a[g][1] = kb + g < num_kb && row + 1 < p.m ? __ldg(a_scale + p.as_sm + (kb + g) * p.as_sk) : 0.f;
+          }
+          if (lane < G::kScaleSteps && kb + lane < num_kb && block * 128 < p.n) b = __ldg(b_scale + (kb + lane) * p.bs_sk);
+          if (!__all_sync(0xffffffffu, mbar_wait(scale_empty_bar + 8 * slot, phase ^ 1u, abort_flag))) {
+            if (lane == 0) give_up(kStatusProducerWait);
+            ok = false;
+            break;
+          }
+          float* to = scale_ring + slot * G::kSlotFloats;
+#pragma unroll
+          for (int g = 0; g < G::kScaleSteps; ++g) *reinterpret_cast<float2*>(to + g * 130 + row_in_tile) = make_float2(a[g][0], a[g][1]);
+          if (lane < G::kScaleSteps) to[lane * 130 + 128 + (warp - 2)] = b;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(scale_full_bar + 8 * slot);
+          if (++slot == G::kScaleSlots) slot = 0, phase ^= 1u;
         }
       }
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t out_buf = smem_base + G::kOutOffset + (warp - 2) * G::kStageOutBytes;
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kManyRegisters));
+    const int quarter = warp & 3, half = (warp - G::kFirstTotalWarp) >> 2;
+    const uint32_t out_buf = smem_base + G::kOutOffset + (warp - G::kFirstTotalWarp) * (G::kOutRows * 128);
+    const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64;
+    int stage = 0, pair = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 0;
     bool ok = true;
     for (int tile = worker; ok && tile < num_tiles; tile += workers) {
       int tm, tn;
       tile_coords(tile, tiles_m, tiles_n, raster_group, tm, tn);
       const int row0 = tm * G::kTile + static_cast<int>(rank) * 128 + quarter * 32;
-      const int row = row0 + lane, col0 = tn * G::kTile + half * 128;
-      const bool live = row < p.m && col0 < p.n;  // (what lies past the matrix is multiplied by zero and never stored)
-      const float* a_scale = p.a_scale + (live ? row * p.as_sm : 0);
-      const float* b_scale = p.b_scale + (live ? col0 / 128 * p.bs_sn : 0);
+      const int col0 = tn * G::kTile + half * 128;
       float2 total[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) total[j] = make_float2(0.f, 0.f);
-      float next_a = live ? __ldg(a_scale) : 0.f, next_b = live ? __ldg(b_scale) : 0.f;
+      float factor[G::kScaleSteps] = {0.f, 0.f, 0.f, 0.f};
       for (int kb = 0; kb < num_kb; ++kb) {
-        const float s = next_a * next_b;
-        if (live && kb + 1 < num_kb) {  // the next step's scales arrive during this one
-          next_a = __ldg(a_scale + (kb + 1) * p.as_sk);
-          next_b = __ldg(b_scale + (kb + 1) * p.bs_sk);
-        }
-        if (!__all_sync(0xffffffffu, mbar_wait_cluster(tmem_full_bar + 8 * acc, acc_phase, abort_flag))) {
-          if (lane == 0) give_up(kStatusEpilogueWait);
-          ok = false;
-          break;
-        }
-        tcgen05_fence_after_sync();
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * G::kTile + half * 128;
-        uint32_t v[2][16];
-        tmem_load_32x16(taddr, v[0]);
-#pragma unroll
-        for (int chunk = 0; chunk < 8; ++chunk) {
-          tmem_load_wait();
-          if (chunk + 1 < 8) {
-            tmem_load_32x16(taddr + 16 * (chunk + 1), v[(chunk + 1) & 1]);
-          } else {
-            tcgen05_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_cta(tmem_empty_bar + 8 * acc, 0));
+        if ((kb & (G::kScaleSteps - 1)) == 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(scale_full_bar + 8 * slot, slot_phase, abort_flag))) {
+            if (lane == 0) give_up(kStatusEpilogueWait);
+            ok = false;
+            break;
           }
+          const float* from = scale_ring + slot * G::kSlotFloats;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f8_fma2(total[8 * chunk + j], v[chunk & 1][2 * j], v[chunk & 1][2 * j + 1], s);
+          for (int g = 0; g < G::kScaleSteps; ++g) factor[g] = from[g * 130 + quarter * 32 + lane] * from[g * 130 + 128 + half];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(scale_empty_bar + 8 * slot);
+          if (++slot == G::kScaleSlots) slot = 0, slot_phase ^= 1u;
         }
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
+        const float s = factor[0];
+#pragma unroll
+        for (int g = 0; g + 1 < G::kScaleSteps; ++g) factor[g] = factor[g + 1];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          if (!__all_sync(0xffffffffu, mbar_wait(done_bar + 16 * stage + 8 * sub, phase, abort_flag))) {
+            if (lane == 0) give_up(kStatusEpilogueWait);
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after_sync();
+          const uint32_t taddr = my_tmem + (2 * pair + sub) * G::kAccColumns;
+          uint32_t v[2][32];
+          tmem_load_32x32(taddr, v[0]);
+          tmem_load_wait();
+          tmem_load_32x32(taddr + 32, v[1]);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) f8_fma2(total[32 * sub + j], v[0][2 * j], v[0][2 * j + 1], s);
+          tmem_load_wait();
+          tcgen05_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(read_bar + 8 * (2 * pair + sub), 0));
+#pragma unroll
+          for (int j = 0; j < 16; ++j) f8_fma2(total[32 * sub + 16 + j], v[1][2 * j], v[1][2 * j + 1], s);
+        }
+        if (!ok) break;
+        if (++stage == G::kStages) stage = 0, phase ^= 1u;
+        pair ^= 1;
       }
       if (!ok) break;
-      // ---- the tile leaves: 128 bytes of every row at a time
+      // ---- the tile leaves: 128 bytes of sixteen rows at a time
       constexpr int kSlabCols = 128 / static_cast<int>(sizeof(OutT));
 #pragma unroll
       for (int slab = 0; slab < 128 / kSlabCols; ++slab) {
         if (col0 + slab * kSlabCols >= p.n || row0 >= p.m) continue;  // (uniform over the warp)
         if (tma_store) {
-          if (lane == 0) tma_store_wait_read<0>();  // the slab before this one has left the buffer
-          __syncwarp();
+          uint32_t w[32];
 #pragma unroll
-          for (int piece = 0; piece < 8; ++piece) {
-            uint32_t w[4];
+          for (int e = 0; e < 32; ++e) {
             if constexpr (sizeof(OutT) == 2) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = total[slab * 32 + piece * 4 + e];
-                w[e] = pack_out16x2<OutT>(f.x, f.y);
-              }
+              const float2 f = total[slab * 32 + e];
+              w[e] = pack_out16x2<OutT>(f.x, f.y);
             } else {
+              const float2 f = total[slab * 16 + e / 2];
+              w[e] = __float_as_uint(e & 1 ? f.y : f.x);
+            }
+          }
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float2 f = total[slab * 16 + piece * 2 + e];
-                w[2 * e] = __float_as_uint(f.x), w[2 * e + 1] = __float_as_uint(f.y);
+          for (int part = 0; part < 32 / G::kOutRows; ++part) {
+            if (lane == 0) tma_store_wait_read<0>();  // the rows before these have left the buffer
+            __syncwarp();
+            if (lane / G::kOutRows == part) {
+#pragma unroll
+              for (int piece = 0; piece < 8; ++piece) {
+                const uint32_t dst = out_buf + (lane % G::kOutRows) * 128 + ((piece ^ (lane & 7)) << 4);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[4 * piece]), "r"(w[4 * piece + 1]), "r"(w[4 * piece + 2]),
+                             "r"(w[4 * piece + 3]) : "memory");
               }
             }
-            const uint32_t dst = out_buf + lane * 128 + ((piece ^ (lane & 7)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              // rows and columns past C are clipped (a store that starts past it would be empty)
+              if (row0 + part * G::kOutRows < p.m) tma_store_2d(&map_c, out_buf, col0 + slab * kSlabCols, row0 + part * G::kOutRows);
+              tma_store_commit();
+            }
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&map_c, out_buf, col0 + slab * kSlabCols, row0);  // rows and columns past C are clipped
-            tma_store_commit();
-          }
-        } else if (row < p.m) {
-          OutT* c = static_cast<OutT*>(p.c) + row * p.c_sm;
+        } else if (row0 + lane < p.m) {
+          OutT* c = static_cast<OutT*>(p.c) + (row0 + lane) * p.c_sm;
 #pragma unroll
           for (int j = 0; j < kSlabCols; ++j) {
             const int col = col0 + slab * kSlabCols + j;

@@ -170,6 +170,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// The same without release: for arrivals that hand over tensor memory whose reads are complete (tcgen05.wait::ld) and no
+// ordinary memory.  A release at cluster scope first waits for every access the thread has in flight, prefetches included.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // ---------------------------------------------------------------- flags between CTAs (global memory)
 
 __device__ __forceinline__ void st_release_gpu_u64(unsigned long long* p, unsigned long long v) {
