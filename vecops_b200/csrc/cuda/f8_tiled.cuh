@@ -76,7 +76,8 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   volatile uint32_t* abort_flag = tmem_slot + 1;
   float* scale_ring = reinterpret_cast<float*>(smem_gen + G::kScaleOffset);  // [slot][step][128 rows of A, 2 blocks of B]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (through a shuffle, so that the compiler knows it to be the same for the whole warp: the roles' loops then run on uniform registers)
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_cta_rank();
   const int worker = static_cast<int>(blockIdx.x >> 1), workers = static_cast<int>(gridDim.x >> 1);
   const int tiles_m = (p.m + G::kTile - 1) / G::kTile, tiles_n = (p.n + G::kTile - 1) / G::kTile;
@@ -140,15 +141,17 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           if (++stage == G::kStages) stage = 0, phase ^= 1u;
         }
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
+      // the whole warp walks the loop, one elected lane issues: what the instructions take stays in uniform registers
       constexpr uint32_t idesc = umma_instr_desc(kUmmaAccF32, kUmmaE4M3, kUmmaE4M3, 256, G::kAccColumns);
+      const bool leader = elect_one();
       int stage = 0, pair = 0;  // pair: accumulators 2 * pair and 2 * pair + 1
       uint32_t phase = 0, pair_phase = 0;
       bool ok = true;
       for (int tile = worker; ok && tile < num_tiles; tile += workers) {
         for (int kb = 0; ok && kb < num_kb; ++kb) {
           if (!mbar_wait(full_bar + 8 * stage, phase, abort_flag)) {
-            give_up(kStatusMmaWaitFull);
+            if (leader) give_up(kStatusMmaWaitFull);
             ok = false;
             break;
           }
@@ -157,15 +160,18 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
           for (int sub = 0; sub < 2; ++sub) {
             if (!mbar_wait(read_bar + 8 * (2 * pair + sub), pair_phase ^ 1u, abort_flag)) {
-              give_up(kStatusMmaWaitTmem);
+              if (leader) give_up(kStatusMmaWaitTmem);
               ok = false;
               break;
             }
             tcgen05_fence_after_sync();
+            if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f8_pair(tmem_base + (2 * pair + sub) * G::kAccColumns, a_desc + 2 * kk, b_desc + sub * (64 * 128 >> 4) + 2 * kk, idesc, kk != 0 ? 1u : 0u);
-            umma_commit_pair(done_bar + 16 * stage + 8 * sub);
+              for (int kk = 0; kk < 4; ++kk)
+                umma_f8_pair(tmem_base + (2 * pair + sub) * G::kAccColumns, a_desc + 2 * kk, b_desc + sub * (64 * 128 >> 4) + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+              umma_commit_pair(done_bar + 16 * stage + 8 * sub);
+            }
+            __syncwarp();
           }
           if (++stage == G::kStages) stage = 0, phase ^= 1u;
           pair ^= 1;
