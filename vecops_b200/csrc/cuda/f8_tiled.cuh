@@ -26,7 +26,7 @@ struct F8Tiled {
   static constexpr int kOperandBytes = 128 * 128;  // 128 rows x 128 bytes of A, and as much of B
   static constexpr int kStageBytes = 2 * kOperandBytes;
   static constexpr int kStages = 6;
-  static constexpr int kAccumulators = 4, kAccColumns = 128;
+  static constexpr int kAccumulators = 2;
   static constexpr int kTotalWarps = 8;
   static constexpr int kFirstTotalWarp = 4;  // register shares are per warpgroup
   static constexpr int kThreads = 32 * (kFirstTotalWarp + kTotalWarps);
@@ -39,7 +39,7 @@ struct F8Tiled {
   static constexpr int kScaleOffset = kOutOffset + kOutBytes;
   static constexpr int kSlotFloats = kScaleSteps * (128 + 2);
   static constexpr int kBarrierOffset = kScaleOffset + kScaleSlots * kSlotFloats * 4;
-  static constexpr int kBarriers = 3 * kStages + kAccumulators + 2 * kScaleSlots;
+  static constexpr int kBarriers = 2 * kStages + kAccumulators + 2 * kScaleSlots;
   static constexpr int kSmemBytes = kBarrierOffset + kBarriers * 8 + 8 + 1024;
   static constexpr int kTmemColumns = 512;
   static constexpr long long kGroupBytes = 32ll << 20;  // raster: row tiles holding this much of A share each sweep over N
@@ -67,9 +67,9 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t full_bar = smem_base + G::kBarrierOffset;        // [stages] both CTAs' tiles landed          (TMA -> MMA; the leader's)
-  const uint32_t done_bar = full_bar + 8 * G::kStages;            // [stages][2] accumulator s of the step ready (MMA -> totals of both;
-                                                                  //             s = 1: the stage is free, too -> TMA of both)
-  const uint32_t read_bar = done_bar + 16 * G::kStages;           // [accumulators] it has been read           (totals of both -> MMA; the leader's)
+  const uint32_t done_bar = full_bar + 8 * G::kStages;            // [stages] a step is multiplied: its sums are ready, its stage is free
+                                                                  //           (MMA -> totals and TMA of both)
+  const uint32_t read_bar = done_bar + 8 * G::kStages;            // [accumulators] read back (totals of both -> MMA; the leader's)
   const uint32_t scale_full_bar = read_bar + 8 * G::kAccumulators;  // [slots]
   const uint32_t scale_empty_bar = scale_full_bar + 8 * G::kScaleSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + G::kBarrierOffset + 8 * G::kBarriers);
@@ -87,8 +87,7 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kStages; ++s) {
       mbar_init(full_bar + 8 * s, 1);
-      mbar_init(done_bar + 16 * s, 1);
-      mbar_init(done_bar + 16 * s + 8, 1);
+      mbar_init(done_bar + 8 * s, 1);
     }
     for (int a = 0; a < G::kAccumulators; ++a) mbar_init(read_bar + 8 * a, 2 * G::kTotalWarps);
     for (int s = 0; s < G::kScaleSlots; ++s) {
@@ -128,7 +127,7 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         int tm, tn;
         tile_coords(tile, tiles_m, tiles_n, raster_group, tm, tn);
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(done_bar + 16 * stage + 8, phase ^ 1u, abort_flag)) {
+          if (!mbar_wait(done_bar + 8 * stage, phase ^ 1u, abort_flag)) {
             give_up(kStatusProducerWait);
             ok = false;
             break;
@@ -143,39 +142,35 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       }
     } else if (warp == 1 && rank == 0) {
       // the whole warp walks the loop, one elected lane issues: what the instructions take stays in uniform registers
-      constexpr uint32_t idesc = umma_instr_desc(kUmmaAccF32, kUmmaE4M3, kUmmaE4M3, 256, G::kAccColumns);
+      constexpr uint32_t idesc = umma_instr_desc(kUmmaAccF32, kUmmaE4M3, kUmmaE4M3, 256, 256);
       const bool leader = elect_one();
-      int stage = 0, pair = 0;  // pair: accumulators 2 * pair and 2 * pair + 1
-      uint32_t phase = 0, pair_phase = 0;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-        for (int kb = 0; ok && kb < num_kb; ++kb) {
+        for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(full_bar + 8 * stage, phase, abort_flag)) {
             if (leader) give_up(kStatusMmaWaitFull);
             ok = false;
             break;
           }
+          if (!mbar_wait(read_bar + 8 * acc, acc_phase ^ 1u, abort_flag)) {
+            if (leader) give_up(kStatusMmaWaitTmem);
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after_sync();
           const uint64_t a_desc = umma_smem_desc_sw128(smem_base + stage * G::kStageBytes);
           const uint64_t b_desc = umma_smem_desc_sw128(smem_base + stage * G::kStageBytes + G::kOperandBytes);
+          if (leader) {
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {
-            if (!mbar_wait(read_bar + 8 * (2 * pair + sub), pair_phase ^ 1u, abort_flag)) {
-              if (leader) give_up(kStatusMmaWaitTmem);
-              ok = false;
-              break;
-            }
-            tcgen05_fence_after_sync();
-            if (leader) {
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                umma_f8_pair(tmem_base + (2 * pair + sub) * G::kAccColumns, a_desc + 2 * kk, b_desc + sub * (64 * 128 >> 4) + 2 * kk, idesc, kk != 0 ? 1u : 0u);
-              umma_commit_pair(done_bar + 16 * stage + 8 * sub);
-            }
-            __syncwarp();
+            for (int kk = 0; kk < 4; ++kk) umma_f8_pair(tmem_base + acc * G::kTile, a_desc + 2 * kk, b_desc + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+            umma_commit_pair(done_bar + 8 * stage);
           }
+          __syncwarp();
           if (++stage == G::kStages) stage = 0, phase ^= 1u;
-          pair ^= 1;
-          if (pair == 0) pair_phase ^= 1u;
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1u;
         }
       }
     } else if (warp >= 2) {
@@ -217,8 +212,8 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kManyRegisters));
     const int quarter = warp & 3, half = (warp - G::kFirstTotalWarp) >> 2;
     const uint32_t out_buf = smem_base + G::kOutOffset + (warp - G::kFirstTotalWarp) * (G::kOutRows * 128);
-    const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64;
-    int stage = 0, pair = 0, slot = 0;
+    const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+    int stage = 0, acc = 0, slot = 0;
     uint32_t phase = 0, slot_phase = 0;
     bool ok = true;
     for (int tile = worker; ok && tile < num_tiles; tile += workers) {
@@ -247,31 +242,30 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const float s = factor[0];
 #pragma unroll
         for (int g = 0; g + 1 < G::kScaleSteps; ++g) factor[g] = factor[g + 1];
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          if (!__all_sync(0xffffffffu, mbar_wait(done_bar + 16 * stage + 8 * sub, phase, abort_flag))) {
-            if (lane == 0) give_up(kStatusEpilogueWait);
-            ok = false;
-            break;
-          }
-          tcgen05_fence_after_sync();
-          const uint32_t taddr = my_tmem + (2 * pair + sub) * G::kAccColumns;
-          uint32_t v[2][32];
-          tmem_load_32x32(taddr, v[0]);
-          tmem_load_wait();
-          tmem_load_32x32(taddr + 32, v[1]);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) f8_fma2(total[32 * sub + j], v[0][2 * j], v[0][2 * j + 1], s);
-          tmem_load_wait();
-          tcgen05_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(read_bar + 8 * (2 * pair + sub), 0));
-#pragma unroll
-          for (int j = 0; j < 16; ++j) f8_fma2(total[32 * sub + 16 + j], v[1][2 * j], v[1][2 * j + 1], s);
+        if (!__all_sync(0xffffffffu, mbar_wait(done_bar + 8 * stage, phase, abort_flag))) {
+          if (lane == 0) give_up(kStatusEpilogueWait);
+          ok = false;
+          break;
         }
-        if (!ok) break;
+        tcgen05_fence_after_sync();
+        const uint32_t taddr = my_tmem + acc * G::kTile;
+        uint32_t v[2][16];
+        tmem_load_32x16(taddr, v[0]);
+#pragma unroll
+        for (int chunk = 0; chunk < 8; ++chunk) {
+          tmem_load_wait();
+          if (chunk + 1 < 8) {
+            tmem_load_32x16(taddr + 16 * (chunk + 1), v[(chunk + 1) & 1]);
+          } else {
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(read_bar + 8 * acc, 0));
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f8_fma2(total[8 * chunk + j], v[chunk & 1][2 * j], v[chunk & 1][2 * j + 1], s);
+        }
         if (++stage == G::kStages) stage = 0, phase ^= 1u;
-        pair ^= 1;
+        acc ^= 1;
       }
       if (!ok) break;
       // ---- the tile leaves: 128 bytes of sixteen rows at a time
