@@ -59,7 +59,7 @@ VECOPS_B200_EXPORT int32_t vecops_b200_quantize_blocks(const VecopsB200QuantizeB
 typedef enum VecopsB200MatmulF8Kernel {
   VECOPS_B200_F8_AUTO = 0,
   VECOPS_B200_F8_GENERIC = 1, /* CUDA cores; any strides */
-  VECOPS_B200_F8_STREAM = 2,  /* few rows of A: weights streamed once through tcgen05 as its 128-row operand */
+  VECOPS_B200_F8_STREAM = 2,  /* up to 128 rows of A: weights streamed once through tcgen05 as its 128-row operand */
   VECOPS_B200_F8_TILED = 3,   /* tcgen05 kind::f8f6f4 on 256 x 256 tiles of CTA pairs */
   VECOPS_B200_F8_COUNT_ = 4
 } VecopsB200MatmulF8Kernel;

@@ -62,7 +62,7 @@ bool f8_addressable(const VecopsB200MatmulF8& p) {
   return p.k > 0 && rows(p.a, p.m, p.a_stride_m, p.a_stride_k) && rows(p.b, p.n, p.b_stride_n, p.b_stride_k);
 }
 
-constexpr int64_t kStreamRows = 256;  // rows of A the streaming kernel holds at most
+constexpr int64_t kStreamRows = 128;  // rows of A the streaming kernel holds at most
 
 int32_t select_f8(const VecopsB200MatmulF8& p, uint32_t* kernel, VecopsError* error) {
   const bool addressable = f8_addressable(p);
@@ -115,6 +115,28 @@ cudaError_t launch_f8(const void* kernel, unsigned grid, int threads, int smem, 
   return cudaLaunchKernelExC(&config, kernel, args);
 }
 
+// How many clusters of `cluster` CTAs of the tiled kernel (all its variants take the same resources) run at once.
+int resident_clusters(const void* kernel, int threads, int smem, int cluster, int device) {
+  static std::atomic<int> known[64][4];  // [device][log2 of the cluster], the count plus one
+  const int bits = cluster == 8 ? 3 : cluster == 4 ? 2 : 1;
+  if (device >= 0 && device < 64 && known[device][bits].load() > 0) return known[device][bits].load() - 1;
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(cluster);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.gridDim = dim3(static_cast<unsigned>(cluster));
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = static_cast<size_t>(smem);
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) clusters = 0;
+  (void)cudaGetLastError();
+  if (device >= 0 && device < 64) known[device][bits].store(clusters + 1);
+  return clusters;
+}
+
 template <int kCols, typename OutT>
 int32_t run_stream_typed(const VecopsB200MatmulF8& q, const DecodeDevice& device, VecopsError* error) {
   using G = F8Stream<kCols>;
@@ -127,13 +149,14 @@ int32_t run_stream_typed(const VecopsB200MatmulF8& q, const DecodeDevice& device
   if (rc != VECOPS_STATUS_OK) return rc;
   rc = f8_operand_map(&map_x, q.a, q.m, q.k, q.a_stride_m, G::kCols, error);
   if (rc != VECOPS_STATUS_OK) return rc;
-  // as many slices of K as one wave of CTAs has room for, each at least two blocks long
+  // as many slices of K as there are SMs for, each at least two blocks long
   const int64_t tiles = (q.n + G::kRows - 1) / G::kRows, blocks = (q.k + 127) / 128;
-  int slices = 1;
-  while (slices < 8 && tiles * slices * 2 <= static_cast<int64_t>(device.sms) * G::kCtasPerSm && blocks >= 2 * 2 * slices) slices *= 2;
+  int slice_bits = 0;
+  while (slice_bits < 3 && (tiles << (slice_bits + 1)) <= device.sms && blocks >= (4 << slice_bits)) ++slice_bits;
+  const int slices = 1 << slice_bits;
   if (tiles * slices > 0x7fffffff) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "matmul_f8: N out of range");
   F8StreamArgs p = f8_args(q, device.status);
-  void* args[] = {&map_w, &map_x, &p, &slices};
+  void* args[] = {&map_w, &map_x, &p, &slice_bits};
   const cudaError_t status = launch_f8(kernel, static_cast<unsigned>(tiles * slices), G::kThreads, G::kSmemBytes, slices, static_cast<cudaStream_t>(q.stream), args);
   if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "matmul_f8 (stream) launch: %s", cudaGetErrorString(status));
   return decode_launched("matmul_f8 (stream)", error);
@@ -144,8 +167,7 @@ int32_t run_stream(const VecopsB200MatmulF8& q, const DecodeDevice& device, Veco
   if (q.m <= 16) return run_stream_typed<16, OutT>(q, device, error);
   if (q.m <= 32) return run_stream_typed<32, OutT>(q, device, error);
   if (q.m <= 64) return run_stream_typed<64, OutT>(q, device, error);
-  if (q.m <= 128) return run_stream_typed<128, OutT>(q, device, error);
-  return run_stream_typed<256, OutT>(q, device, error);
+  return run_stream_typed<128, OutT>(q, device, error);
 }
 
 template <typename OutT>
@@ -174,12 +196,15 @@ int32_t run_tiled(const VecopsB200MatmulF8& q, const DecodeDevice& device, Vecop
   }
   const int64_t tiles_m = (q.m + G::kTile - 1) / G::kTile, tiles_n = (q.n + G::kTile - 1) / G::kTile;
   if (tiles_m * tiles_n > 0x7fffffff) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "matmul_f8: too many tiles");
-  const int64_t workers = tiles_m * tiles_n < device.sms / 2 ? tiles_m * tiles_n : device.sms / 2;
+  const int64_t tiles = tiles_m * tiles_n, blocks = (q.k + 127) / 128;
+  int slice_bits = 0;
+  while (slice_bits < 2 && blocks >= (8 << slice_bits) && tiles <= resident_clusters(kernel, G::kThreads, G::kSmemBytes, 4 << slice_bits, device.index)) ++slice_bits;
+  const int64_t workers = tiles < device.sms / 2 ? tiles : device.sms / 2;
   const int64_t group = G::kGroupBytes / (static_cast<int64_t>(G::kTile) * (q.k < 1 ? 1 : q.k));
   int raster_group = static_cast<int>(group < 1 ? 1 : group < tiles_m ? group : tiles_m);
   F8StreamArgs p = f8_args(q, device.status);
-  void* args[] = {&map_a, &map_b, &map_c, &p, &tma_store, &raster_group};
-  const cudaError_t status = launch_f8(kernel, static_cast<unsigned>(2 * workers), G::kThreads, G::kSmemBytes, 2, static_cast<cudaStream_t>(q.stream), args);
+  void* args[] = {&map_a, &map_b, &map_c, &p, &tma_store, &raster_group, &slice_bits};
+  const cudaError_t status = launch_f8(kernel, static_cast<unsigned>(2 * workers << slice_bits), G::kThreads, G::kSmemBytes, 2 << slice_bits, static_cast<cudaStream_t>(q.stream), args);
   if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "matmul_f8 (tiled) launch: %s", cudaGetErrorString(status));
   return decode_launched("matmul_f8 (tiled)", error);
 }

@@ -4,17 +4,18 @@
 //
 // A block's scales apply to its sum over 128 k, so every 128-k step of the main loop is an accumulation of its own, which
 // eight warps read back from tensor memory and add, scaled, to totals in registers while the tensor cores work on the next.
-// What bounds the kernel is the round trip MMA -> commit -> read-back -> arrival -> MMA of one accumulator, so tensor
-// memory is cut into four accumulators of 128 columns (two per step) rather than two of 256: three are in flight while
-// one is read.  Roles, per CTA:
+// Four MMAs of 256 columns take 512 cycles; the round trip MMA -> commit -> read-back -> arrival -> MMA of an
+// accumulator is what keeps the kernel from that rate, as tensor memory holds two of them.  (Four accumulators of 128
+// columns hide it better, but an MMA of 128 columns takes 80 cycles, not 64, and measured 12 % slower; shared memory,
+// which the MMAs and the arriving tiles keep busy, makes every barrier slow, too.)  Roles, per CTA:
 //   warp 0      TMA: its 128 rows of A and its 128 of the tile's 256 rows of B per step, a ring of kStages
 //   warp 1      (leader CTA) issues tcgen05.mma.cta_group::2, M = 256, N = 128, four of 32 k per accumulator
 //   warps 2-3   fetch the scales into a ring in shared memory, up to 32 steps ahead (fetched by the totals' own threads, 32
 //               rows a warp and each in a line of its own, they took as long as the product itself)
 //   warps 4-11  totals - a thread owns one row and 128 columns of C, all of one weight block: one factor sa * sb per step
 //               and one fused multiply-add per element, two per instruction - then the store of the tile by TMA
-// Of a pair MMA with N = 128 each CTA feeds 64 rows of B: accumulator s of a step holds the tile's columns [64 s, 64 s + 64)
-// and [128 + 64 s, 128 + 64 s + 64).  Persistent: pairs walk the tiles `worker, worker + workers, ...`.
+// Persistent: pairs walk the tiles `worker, worker + workers, ...`.  With fewer tiles than pairs, K is cut into 2 or 4 slices:
+// the pairs of a tile's slices form a cluster, and each of its CTAs sums a share of the rows through the others' shared memory.
 #pragma once
 
 #include "f8_stream.cuh"
@@ -42,9 +43,11 @@ struct F8Tiled {
   static constexpr int kBarriers = 2 * kStages + kAccumulators + 2 * kScaleSlots;
   static constexpr int kSmemBytes = kBarrierOffset + kBarriers * 8 + 8 + 1024;
   static constexpr int kTmemColumns = 512;
+  static constexpr int kMaxSlices = 4;  // pairs of one cluster, 8 CTAs
   static constexpr long long kGroupBytes = 32ll << 20;  // raster: row tiles holding this much of A share each sweep over N
 };
 static_assert((F8Tiled::kFewRegisters + 2 * F8Tiled::kManyRegisters) * 128 <= 168 * F8Tiled::kThreads, "register split");
+static_assert(128 * 1024 <= F8Tiled::kStages * F8Tiled::kStageBytes, "the totals of a slice are left over the ring");
 static_assert(F8Tiled::kSmemBytes <= 227 * 1024, "shared memory budget");
 static_assert(F8Tiled::kBarrierOffset % 8 == 0, "barriers are 8-byte words");
 
@@ -61,7 +64,7 @@ __device__ __forceinline__ void f8_fma2(float2& acc, uint32_t v0, uint32_t v1, f
 template <typename OutT>
 __global__ void __launch_bounds__(F8Tiled::kThreads, 1)
 f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
-                const F8StreamArgs p, int tma_store, int raster_group) {
+                const F8StreamArgs p, int tma_store, int raster_group, int slice_bits) {
   using G = F8Tiled;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -78,11 +81,15 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 
   // (through a shuffle, so that the compiler knows it to be the same for the whole warp: the roles' loops then run on uniform registers)
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_cta_rank();
-  const int worker = static_cast<int>(blockIdx.x >> 1), workers = static_cast<int>(gridDim.x >> 1);
+  const uint32_t cluster_rank = cluster_cta_rank(), rank = cluster_rank & 1u, leader_rank = cluster_rank & ~1u;
+  const uint16_t both = static_cast<uint16_t>(3u << leader_rank);
+  const int slice = static_cast<int>(cluster_rank >> 1);
+  const int worker = static_cast<int>(blockIdx.x >> (1 + slice_bits)), workers = static_cast<int>(gridDim.x >> (1 + slice_bits));
   const int tiles_m = (p.m + G::kTile - 1) / G::kTile, tiles_n = (p.n + G::kTile - 1) / G::kTile;
   const int num_tiles = tiles_m * tiles_n;
-  const int num_kb = (p.k + 127) / 128;
+  const int all_kb = (p.k + 127) / 128;
+  const int kb_begin = static_cast<int>(static_cast<long long>(all_kb) * slice >> slice_bits);
+  const int num_kb = static_cast<int>(static_cast<long long>(all_kb) * (slice + 1) >> slice_bits) - kb_begin;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kStages; ++s) {
@@ -133,10 +140,10 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             break;
           }
           const uint32_t a_dst = smem_base + stage * G::kStageBytes;
-          const uint32_t leader_full = map_to_cta(full_bar + 8 * stage, 0);
+          const uint32_t leader_full = map_to_cta(full_bar + 8 * stage, leader_rank);
           if (rank == 0) mbar_arrive_expect_tx(full_bar + 8 * stage, 2 * G::kStageBytes);
-          tma_load_2d_pair(a_dst, &map_a, leader_full, kb * 128, tm * G::kTile + static_cast<int>(rank) * 128);
-          tma_load_2d_pair(a_dst + G::kOperandBytes, &map_b, leader_full, kb * 128, tn * G::kTile + static_cast<int>(rank) * 128);
+          tma_load_2d_pair(a_dst, &map_a, leader_full, (kb_begin + kb) * 128, tm * G::kTile + static_cast<int>(rank) * 128);
+          tma_load_2d_pair(a_dst + G::kOperandBytes, &map_b, leader_full, (kb_begin + kb) * 128, tn * G::kTile + static_cast<int>(rank) * 128);
           if (++stage == G::kStages) stage = 0, phase ^= 1u;
         }
       }
@@ -165,7 +172,7 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           if (leader) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) umma_f8_pair(tmem_base + acc * G::kTile, a_desc + 2 * kk, b_desc + 2 * kk, idesc, kk != 0 ? 1u : 0u);
-            umma_commit_pair(done_bar + 8 * stage);
+            umma_commit_pair_of(done_bar + 8 * stage, both);
           }
           __syncwarp();
           if (++stage == G::kStages) stage = 0, phase ^= 1u;
@@ -183,8 +190,8 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         tile_coords(tile, tiles_m, tiles_n, raster_group, tm, tn);
         const int row = tm * G::kTile + static_cast<int>(rank) * 128 + row_in_tile;
         const int block = 2 * tn + (warp - 2);  // weight block fetched by lanes 0..3 of the warp, one step each
-        const float* a_scale = p.a_scale + static_cast<long long>(row) * p.as_sm;
-        const float* b_scale = p.b_scale + static_cast<long long>(block) * p.bs_sn;
+        const float* a_scale = p.a_scale + static_cast<long long>(row) * p.as_sm + kb_begin * p.as_sk;
+        const float* b_scale = p.b_scale + static_cast<long long>(block) * p.bs_sn + kb_begin * p.bs_sk;
         for (int kb = 0; kb < num_kb; kb += G::kScaleSteps) {
           float a[G::kScaleSteps][2], b = 0.f;
 #pragma unroll
@@ -259,7 +266,7 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           } else {
             tcgen05_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(read_bar + 8 * acc, 0));
+            if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(read_bar + 8 * acc, leader_rank));
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) f8_fma2(total[8 * chunk + j], v[chunk & 1][2 * j], v[chunk & 1][2 * j + 1], s);
@@ -268,6 +275,18 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         acc ^= 1;
       }
       if (!ok) break;
+      if (slice_bits > 0) {
+        // every MMA of this CTA is done and has read what TMA brought: the totals go over the ring as rows of 256 floats, their
+        // 16-byte pieces swizzled by the row so that neither these stores nor the reads below meet in a bank
+        const int row = quarter * 32 + lane;
+#pragma unroll
+        for (int piece = 0; piece < 32; ++piece) {
+          const uint32_t dst = smem_base + row * 1024 + (((half * 32 + piece) ^ (row & 7)) << 4);
+          const float2 x = total[2 * piece], y = total[2 * piece + 1];
+          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y) : "memory");
+        }
+        break;  // (one tile per cluster)
+      }
       // ---- the tile leaves: 128 bytes of sixteen rows at a time
       constexpr int kSlabCols = 128 / static_cast<int>(sizeof(OutT));
 #pragma unroll
@@ -317,6 +336,24 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       }
     }
     if (lane == 0) tma_store_wait_all<0>();
+  }
+
+  __syncthreads();
+  if (slice_bits > 0) {
+    // ---- the slices of the tile meet: this CTA sums every 2^slice_bits-th of its 128 rows, in slice order
+    cluster_sync_all();
+    if (*abort_flag == 0) {
+      int tm, tn;
+      tile_coords(worker, tiles_m, tiles_n, raster_group, tm, tn);
+      const bool wide = f8_wide_store(p);
+      const int first_row = tm * G::kTile + static_cast<int>(rank) * 128;
+      for (int item = warp; item < 256 >> slice_bits; item += G::kThreads / 32) {  // half a row each
+        const int row = slice + (item >> 1 << slice_bits), piece = (item & 1) * 32 + lane;
+        if (first_row + row >= p.m) break;
+        const float4 sum = f8_sum_slices<G::kMaxSlices>(smem_base + row * 1024 + ((piece ^ (row & 7)) << 4), 1 << slice_bits, static_cast<int>(rank), 2);
+        f8_store4<OutT>(p, first_row + row, tn * G::kTile + 4 * piece, sum, wide);
+      }
+    }
   }
 
   // ---------------------------------------------------------------- teardown

@@ -149,10 +149,6 @@ __device__ __forceinline__ void cluster_sync_all() {
                "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The two halves of the same barrier, for work that fits between them.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 // Read one float from another CTA's shared memory (`cluster_addr` from map_to_cta).
 __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
   float value;
@@ -160,9 +156,10 @@ __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
   return value;
 }
 
-// Write one float into another CTA's shared memory (`cluster_addr` from map_to_cta).
-__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float value) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(value) : "memory");
+__device__ __forceinline__ float4 ld_shared_cluster_v4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
 }
 
 // Arrive on a barrier that may live in the peer CTA (`cluster_addr` from map_to_cta).
@@ -417,6 +414,13 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t a_desc, u
 // far has finished.  (An arrival on barriers, not a data transfer: no load is involved.)
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
   const uint16_t both = 3;
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"(both)
+               : "memory");
+}
+
+// The same for a pair inside a larger cluster: `both` has the bits of its two ranks.
+__device__ __forceinline__ void umma_commit_pair_of(uint32_t bar, uint16_t both) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
                "h"(both)
                : "memory");
