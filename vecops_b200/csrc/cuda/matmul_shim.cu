@@ -1176,12 +1176,12 @@ int32_t launch_f32(const VecopsB200Matmul& p, cudaStream_t stream, VecopsError* 
 
 int32_t shim_encode_map(CUtensorMap* out, CUtensorMapDataType dtype, uint32_t rank, const void* base, const uint64_t* dims,
                         const uint64_t* strides_bytes, const uint32_t* box, VecopsError* error) {
-  if (rank < 2 || rank > 3) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "tensor map rank %u not served", rank);
+  if (rank < 2 || rank > 4) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "tensor map rank %u not served", rank);
   if (g_encode_tiled == nullptr) return set_error(error, VECOPS_STATUS_LOAD_ERROR, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t d[3] = {dims[0], dims[1], rank > 2 ? dims[2] : 1};
-  cuuint64_t s[2] = {strides_bytes[0], rank > 2 ? strides_bytes[1] : 0};
-  cuuint32_t b[3] = {box[0], box[1], rank > 2 ? box[2] : 1};
-  cuuint32_t e[3] = {1, 1, 1};
+  cuuint64_t d[4] = {dims[0], dims[1], rank > 2 ? dims[2] : 1, rank > 3 ? dims[3] : 1};
+  cuuint64_t s[3] = {strides_bytes[0], rank > 2 ? strides_bytes[1] : 0, rank > 3 ? strides_bytes[2] : 0};
+  cuuint32_t b[4] = {box[0], box[1], rank > 2 ? box[2] : 1, rank > 3 ? box[3] : 1};
+  cuuint32_t e[4] = {1, 1, 1, 1};
   const CUresult result = g_encode_tiled(out, dtype, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (result != CUDA_SUCCESS)

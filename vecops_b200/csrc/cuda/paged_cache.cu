@@ -2,9 +2,13 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "cache_append.cuh"
 #include "decode_shim.h"
+#include "prefix_sdpa.cuh"
 #include "prefix_sdpa_generic.cuh"
+#include "suffix_sdpa.cuh"
 
 using namespace vb200;
 
@@ -88,6 +92,141 @@ PrefixSdpaArgs prefix_args(const VecopsB200PrefixAttention& a) {
   return p;
 }
 
+// ---------------------------------------------------------------- the two-kernel form: prefix on tcgen05, suffix and merge behind it
+
+struct PrefixPlan {
+  bool fast = false;  // the two kernels can address this call; the one-warp-per-row kernel serves the rest
+  int dim = 0;        // head dims a kernel is built for: 64 or 128
+  int both_rows = 0, row_blocks = 0, tiles = 0, tiles_per_chunk = 0, chunks = 0, records = 0;
+  uint64_t ml_at = 0, total = 0;
+};
+
+PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
+  PrefixPlan p;
+  // sixteen-byte loads of every row
+  auto rows_ok = [](const void* base, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2) {
+    return decode_aligned(base, 16) && (n0 <= 1 || s0 % 8 == 0) && (n1 <= 1 || s1 % 8 == 0) && (n2 <= 1 || s2 % 8 == 0);
+  };
+  const bool pages_ok = a.page_size % 128 == 0 || (a.page_size % 8 == 0 && 128 % a.page_size == 0);  // a tile of 128 keys is whole pages or lies in one
+  p.fast = a.head_dim <= 128 && a.head_dim % 8 == 0 && (a.prefix_len == 0 || pages_ok) &&
+           rows_ok(a.q, a.tokens, a.q_stride_token, a.q_heads, a.q_stride_head, 1, 0) && rows_ok(a.out, a.tokens, a.out_stride_token, a.q_heads, a.out_stride_head, 1, 0) &&
+           rows_ok(a.k_cache, a.pages, a.k_stride_page, a.page_size, a.k_stride_slot, a.kv_heads, a.k_stride_head) &&
+           rows_ok(a.v_cache, a.pages, a.v_stride_page, a.page_size, a.v_stride_slot, a.kv_heads, a.v_stride_head) &&
+           a.tokens * (a.q_heads / a.kv_heads) < (INT64_C(1) << 31) - 256 && a.kv_heads <= 65535;
+  if (!p.fast) return p;
+  p.dim = a.head_dim <= 64 ? 64 : 128;
+  if (a.prefix_len == 0 || a.tokens == 0 || a.pages == 0) return p;
+  const int64_t rows = a.tokens * (a.q_heads / a.kv_heads);
+  p.both_rows = rows > 128 ? 1 : 0;
+  p.row_blocks = static_cast<int>(p.both_rows ? (rows + 255) / 256 : 1);
+  p.tiles = static_cast<int>((a.prefix_len + 127) / 128);
+  // Cut the prefix so that the waves of work items are full: the cost of a cut is its waves times (tiles of an item + what an
+  // item costs besides, about two tiles: Q, the first loads, the records), and one tile's worth per record written.
+  const int64_t base = a.kv_heads * p.row_blocks;
+  int64_t best = 0;
+  for (int chunks = 1; chunks <= p.tiles && chunks <= 128; ++chunks) {
+    const int per_chunk = (p.tiles + chunks - 1) / chunks;
+    const int used = (p.tiles + per_chunk - 1) / per_chunk;
+    const int64_t waves = (base * used + sms - 1) / sms;
+    const int64_t cost = waves * (per_chunk + 2) * 64 + waves * 32 * (used > 1 ? 1 : 0);
+    if (best == 0 || cost < best) best = cost, p.tiles_per_chunk = per_chunk, p.chunks = used;
+  }
+  p.records = p.both_rows ? p.chunks : 2 * p.chunks;
+  const uint64_t record_rows = static_cast<uint64_t>(p.records) * a.kv_heads * rows;
+  p.ml_at = record_rows * p.dim * 4;
+  p.total = p.ml_at + record_rows * 8;
+  return p;
+}
+
+template <typename T, int kDim>
+int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, const DecodeDevice& device, VecopsError* error) {
+  using G = PrefixTc<kDim>;
+  const PrefixSdpaArgs args = prefix_args(a);
+  cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.stream = stream;
+  config.attrs = attributes;
+  static std::atomic<bool> raised[64];
+  if (device.index >= 64 || !raised[device.index].load()) {
+    cudaError_t status = cudaFuncSetAttribute(prefix_sdpa_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmemBytes);
+    if (status == cudaSuccess) status = cudaFuncSetAttribute(suffix_sdpa_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, SuffixSdpa<kDim>::kSmemBytes);
+    if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "cudaFuncSetAttribute(prefix_sdpa): %s", cudaGetErrorString(status));
+    if (device.index < 64) raised[device.index].store(true);
+  }
+  const int rows = static_cast<int>(a.tokens * (a.q_heads / a.kv_heads));
+  float* partial_o = static_cast<float*>(a.workspace);
+  float2* partial_ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + plan.ml_at);
+  if (plan.records > 0) {
+    PrefixTcArgs p{};
+    p.a = args;
+    p.rows = rows, p.row_blocks = plan.row_blocks, p.tiles = plan.tiles, p.tiles_per_chunk = plan.tiles_per_chunk, p.both_rows = plan.both_rows;
+    p.box_keys = static_cast<int>(a.page_size < 128 ? a.page_size : 128);
+    p.partial_o = partial_o, p.partial_ml = partial_ml, p.status = device.status;
+    CUtensorMap map_k, map_v;
+    auto cache_map = [&](CUtensorMap* map, const void* base, int64_t page, int64_t slot, int64_t head) {
+      // (a dimension of one has no stride that matters, but the map wants a legal one)
+      auto bytes = [](int64_t n, int64_t stride) { return static_cast<uint64_t>(n > 1 ? stride * 2 : 16); };
+      const uint64_t dims[4] = {static_cast<uint64_t>(a.head_dim), static_cast<uint64_t>(a.page_size), static_cast<uint64_t>(a.kv_heads), static_cast<uint64_t>(a.pages)};
+      const uint64_t strides[3] = {bytes(a.page_size, slot), bytes(a.kv_heads, head), bytes(a.pages, page)};
+      const uint32_t box[4] = {64, static_cast<uint32_t>(p.box_keys), 1, 1};
+      const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+      return shim_encode_map(map, type, 4, base, dims, strides, box, error);
+    };
+    int32_t rc = cache_map(&map_k, a.k_cache, a.k_stride_page, a.k_stride_slot, a.k_stride_head);
+    if (rc != VECOPS_STATUS_OK) return rc;
+    rc = cache_map(&map_v, a.v_cache, a.v_stride_page, a.v_stride_slot, a.v_stride_head);
+    if (rc != VECOPS_STATUS_OK) return rc;
+    config.gridDim = dim3(static_cast<unsigned>(plan.chunks), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(plan.row_blocks));
+    config.blockDim = dim3(G::kThreads);
+    config.dynamicSmemBytes = G::kSmemBytes;
+    config.numAttrs = 1;
+    const cudaError_t status = cudaLaunchKernelEx(&config, prefix_sdpa_kernel<T, kDim>, map_k, map_v, p);
+    if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "prefix_sdpa launch: %s", cudaGetErrorString(status));
+    rc = decode_launched("prefix_sdpa", error);
+    if (rc != VECOPS_STATUS_OK) return rc;
+  }
+  SuffixSdpaArgs s{};
+  s.a = args;
+  s.rows = rows;
+  s.tokens_per_item = args.group <= 16 ? 16 / args.group : 1;
+  s.group_tiles = (args.group + 15) / 16;
+  s.records = plan.records, s.partial_o = partial_o, s.partial_ml = partial_ml;
+  const int64_t slots = a.query_starts == nullptr ? a.batch : a.tokens / s.tokens_per_item + a.batch + 1;
+  const int64_t items = slots * a.kv_heads * s.group_tiles, capacity = a.table_width * a.page_size;
+  // few items: several CTAs share one, each warp with a slice of sixteen keys at least; two CTAs fit an SM
+  while (s.split_bits < 3 && (items << (s.split_bits + 1)) <= 2 * static_cast<int64_t>(device.sms) && (INT64_C(128) << s.split_bits) <= capacity) ++s.split_bits;
+  if ((slots << s.split_bits) > 0x7fffffff || a.kv_heads * s.group_tiles > 65535)
+    return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
+  s.slots = static_cast<int>(slots);
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = 1u << s.split_bits;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  config.gridDim = dim3(static_cast<unsigned>(slots << s.split_bits), static_cast<unsigned>(a.kv_heads * s.group_tiles));
+  config.blockDim = dim3(SuffixSdpa<kDim>::kThreads);
+  config.dynamicSmemBytes = SuffixSdpa<kDim>::kSmemBytes;
+  config.numAttrs = 2;
+  const cudaError_t status = cudaLaunchKernelEx(&config, suffix_sdpa_kernel<T, kDim>, s);
+  if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "suffix_sdpa launch: %s", cudaGetErrorString(status));
+  return decode_launched("suffix_sdpa", error);
+}
+
+template <typename T>
+int32_t run_prefix_generic(const VecopsB200PrefixAttention& a, VecopsError* error) {
+  const int64_t blocks = (a.tokens * a.q_heads + 7) / 8;
+  if (blocks >= (INT64_C(1) << 31)) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
+  prefix_sdpa_generic_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(a.stream)>>>(prefix_args(a));
+  return decode_launched("prefix_sdpa (generic)", error);
+}
+
+template <typename T>
+int32_t run_prefix_typed(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, const DecodeDevice& device, VecopsError* error) {
+  if (!plan.fast) return run_prefix_generic<T>(a, error);
+  return plan.dim == 64 ? run_prefix<T, 64>(a, plan, device, error) : run_prefix<T, 128>(a, plan, device, error);
+}
+
 }  // namespace
 
 extern "C" {
@@ -137,8 +276,15 @@ int32_t vecops_b200_prefix_sdpa_workspace(const VecopsB200PrefixAttention* atten
   if (attention == nullptr || attention->struct_size < sizeof(VecopsB200PrefixAttention) || bytes == nullptr)
     return set_error(error, VECOPS_STATUS_ABI_MISMATCH, "prefix attention record is null or too small, or no output pointer");
   const int32_t rc = check_prefix(*attention, error);
-  if (rc == VECOPS_STATUS_OK) *bytes = 0;
-  return rc;
+  if (rc != VECOPS_STATUS_OK) return rc;
+  // the SM count of the device the record names, or of a B200 when no device can be asked
+  int sms = 148, device = attention->device_index;
+  if (vecops_b200_device_count() > 0 && (device >= 0 || cudaGetDevice(&device) == cudaSuccess)) {
+    int asked = 0;
+    if (shim_device_facts(device, &asked, nullptr, nullptr, nullptr) == VECOPS_STATUS_OK && asked > 0) sms = asked;
+  }
+  *bytes = plan_prefix(*attention, sms).total;
+  return VECOPS_STATUS_OK;
 }
 
 int32_t vecops_b200_prefix_sdpa_run(const VecopsB200PrefixAttention* attention, VecopsError* error) {
@@ -152,13 +298,11 @@ int32_t vecops_b200_prefix_sdpa_run(const VecopsB200PrefixAttention* attention, 
   DecodeDevice device;
   rc = decode_enter(a.device_index, &device, error);
   if (rc != VECOPS_STATUS_OK) return rc;
-  const PrefixSdpaArgs p = prefix_args(a);
-  const int64_t blocks = (a.tokens * a.q_heads + 7) / 8;
-  if (blocks >= (INT64_C(1) << 31)) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
-  cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
-  if (a.dtype == VECOPS_DTYPE_BF16) prefix_sdpa_generic_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
-  else prefix_sdpa_generic_kernel<__half><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
-  rc = decode_launched("prefix_sdpa (generic)", error);
+  const PrefixPlan plan = plan_prefix(a, device.sms);
+  if (plan.total != 0 && (a.workspace == nullptr || !decode_aligned(a.workspace, 256) || a.workspace_size < plan.total))
+    return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa needs %llu bytes of 256-byte aligned device scratch (vecops_b200_prefix_sdpa_workspace)",
+                     (unsigned long long)plan.total);
+  rc = a.dtype == VECOPS_DTYPE_BF16 ? run_prefix_typed<__nv_bfloat16>(a, plan, device, error) : run_prefix_typed<__half>(a, plan, device, error);
   if (rc != VECOPS_STATUS_OK) return rc;
   return decode_finish("prefix_sdpa", a.flags, a.stream, device.index, error);
 }

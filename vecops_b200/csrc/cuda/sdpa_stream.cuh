@@ -95,12 +95,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // kPlain: no key mask, no two-dimensional keep mask, no bias (the query mask and the causal cut cost nothing).
 template <bool kPlain, bool kTrace = false>
 __global__ void __launch_bounds__(SdpaStream::kThreads, 1)

@@ -8,7 +8,7 @@
 
 namespace vb200 {
 
-// Tiled tensor map with the 128-byte swizzle over a tensor of `rank` (2 or 3) dimensions, innermost first:
+// Tiled tensor map with the 128-byte swizzle over a tensor of `rank` (2 to 4) dimensions, innermost first:
 // dims[rank], strides_bytes[rank - 1] (dimension 0 is contiguous), box[rank].
 int32_t shim_encode_map(CUtensorMap* out, CUtensorMapDataType dtype, uint32_t rank, const void* base, const uint64_t* dims,
                         const uint64_t* strides_bytes, const uint32_t* box, VecopsError* error);
