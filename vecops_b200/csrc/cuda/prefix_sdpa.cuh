@@ -40,11 +40,9 @@ struct PrefixTc {
   static constexpr int kBarriers = 2 * kSlots + 5;
   static constexpr int kSmemBytes = kBarrierOffset + kBarriers * 8 + 16 + 1024;
   static constexpr int kThreads = 384;
-  static constexpr int kFewRegisters = 56, kManyRegisters = 224;
   static constexpr int kTmemColumns = 512;               // group g: scores (and probabilities over them) at 256 g, O at 256 g + 128
 };
 static_assert(PrefixTc<128>::kSmemBytes <= 227 * 1024 && PrefixTc<64>::kSmemBytes <= 227 * 1024, "shared memory budget");
-static_assert((PrefixTc<128>::kFewRegisters + 2 * PrefixTc<128>::kManyRegisters) * 128 <= 168 * PrefixTc<128>::kThreads, "register split");
 
 struct PrefixTcArgs {
   PrefixSdpaArgs a;
@@ -122,7 +120,6 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kFewRegisters));
     if (warp == 0) {
       // ---------------------------------------------------------------- pages and TMA: a lane per page of the tile
       const int boxes = G::kKeys / p.box_keys;
@@ -270,22 +267,33 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     }
   } else {
     // ---------------------------------------------------------------- softmax: a thread per row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kManyRegisters));
     const int g = (warp - 4) >> 2, quarter = warp & 3;
     const int thread = static_cast<int>(threadIdx.x) - 128;
     {
       // Q: rows of 16-byte pieces under the 128-byte swizzle; rows past the last and dims past head_dim are zero
-      constexpr int kPieces = kDim / 8;
-      const int q_rows = p.both_rows ? 2 * G::kRows : G::kRows;
-      for (int i = thread; i < q_rows * kPieces; i += 256) {
-        const int row = i / kPieces, piece = i % kPieces, r = row0 + row;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < p.rows && piece * 8 < p.a.head_dim) {
-          const int t = r / p.a.group, head = kv * p.a.group + r % p.a.group;
-          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + t * p.a.q_st + head * p.a.q_sh + piece * 8);
+      // (eight rows' loads in flight together)
+      constexpr int kPieces = kDim / 8, kRowStep = 256 / kPieces, kTogether = 8;
+      const int piece = thread % kPieces;
+      const bool in_head = piece * 8 < p.a.head_dim;
+#pragma unroll 1
+      for (int first = thread / kPieces; first < (p.both_rows ? 2 * G::kRows : G::kRows); first += kRowStep * kTogether) {
+        uint4 x[kTogether];
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+          const int r = row0 + first + i * kRowStep;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (r < p.rows && in_head) {
+            const int t = r / p.a.group, head = kv * p.a.group + r - t * p.a.group;
+            x[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + t * p.a.q_st + head * p.a.q_sh + piece * 8));
+          }
         }
-        const uint32_t dst = smem_base + G::kQOffset + (row >> 7) * G::kTileBytes + (piece >> 3) * G::kAtomBytes + (row & 127) * 128 + (((piece & 7) ^ (row & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+          const int row = first + i * kRowStep;
+          const uint32_t dst = smem_base + G::kQOffset + (row >> 7) * G::kTileBytes + (piece >> 3) * G::kAtomBytes + (row & 127) * 128 + (((piece & 7) ^ (row & 7)) << 4);
+          if (row < (p.both_rows ? 2 * G::kRows : G::kRows))
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z), "r"(x[i].w) : "memory");
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -309,29 +317,36 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     for (int tile = p.both_rows ? 0 : g; ok && tile < n; tile += p.both_rows ? 1 : 2, ++turn) {
       wait_scores();
       if (!ok) break;
-      float t[128];
-      {
-        uint32_t* v = reinterpret_cast<uint32_t*>(t);
-        tmem_load_32x64(my_tmem, *reinterpret_cast<uint32_t(*)[64]>(v));
-        tmem_load_32x64(my_tmem + 64, *reinterpret_cast<uint32_t(*)[64]>(v + 64));
-        tmem_load_wait();
-      }
-      if (signed_scale <= 0.f) {  // (so that the factor below is positive: the maximum, and a masked -inf, keep their meaning)
-        const float sign = signed_scale < 0.f ? -1.f : 0.f;
-#pragma unroll
-        for (int j = 0; j < 128; ++j) t[j] *= sign;
-      }
+      // Two passes over the scores where they lie, 32 columns at a time: the maximum, then the probabilities, which go over
+      // columns already read.  (128 scores held in registers instead spilled, and the code, unrolled, took longer to fetch
+      // than a short item takes to run.)
       const int last = p.a.prefix_len - (first_tile + tile) * G::kKeys;
       const uint32_t gone = absent[tile % G::kMaskSlots];
-      if (last < G::kKeys || gone != 0) {
+      const bool cut = last < G::kKeys || gone != 0;  // (the same for the whole item)
+      auto load_scores = [&](int col, float (&t)[32]) {
+        tmem_load_32x32(my_tmem + col, reinterpret_cast<uint32_t(&)[32]>(t));
+        tmem_load_wait();
+        if (signed_scale <= 0.f) {  // (so that the factor below is positive: the maximum, and a masked -inf, keep their meaning)
+          const float sign = signed_scale < 0.f ? -1.f : 0.f;
 #pragma unroll
-        for (int j = 0; j < 128; ++j)
-          if (j >= last || (gone >> (j >> box_shift) & 1u) != 0) t[j] = -INFINITY;
+          for (int j = 0; j < 32; ++j) t[j] *= sign;
+        }
+        if (cut) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col + j >= last || (gone >> ((col + j) >> box_shift) & 1u) != 0) t[j] = -INFINITY;
+        }
+      };
+      float highest = -INFINITY;
+#pragma unroll 1
+      for (int col = 0; col < 128; col += 32) {
+        float t[32];
+        load_scores(col, t);
+        float top[4] = {t[0], t[1], t[2], t[3]};
+#pragma unroll
+        for (int j = 4; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], t[j]);
+        highest = fmaxf(highest, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
       }
-      float top[4] = {t[0], t[1], t[2], t[3]};
-#pragma unroll
-      for (int j = 4; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], t[j]);
-      const float highest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
       const float tile_max = highest * scale;
       const bool moves = turn == 0 || tile_max > m + 8.f;
       if (turn == 0) {
@@ -353,17 +368,19 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       }
       const float m_use = m == -INFINITY ? 0.f : m;  // nothing kept so far: every p is 0
       float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int col = 0; col < 128; col += 32) {
+        float t[32];
+        load_scores(col, t);
+        uint32_t packed[16];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float p0 = exp2_approx(fmaf(t[64 * half + 2 * j], scale, -m_use)), p1 = exp2_approx(fmaf(t[64 * half + 2 * j + 1], scale, -m_use));
+        for (int j = 0; j < 16; ++j) {
+          const float p0 = exp2_approx(fmaf(t[2 * j], scale, -m_use)), p1 = exp2_approx(fmaf(t[2 * j + 1], scale, -m_use));
           sums[(2 * j) & 3] += p0;
           sums[(2 * j + 1) & 3] += p1;
           packed[j] = prefix_pack<T>(p0, p1);
         }
-        tmem_store_32x32(my_tmem + 32 * half, packed);
+        tmem_store_32x16(my_tmem + col / 2, packed);
       }
       l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
       tmem_store_wait();
