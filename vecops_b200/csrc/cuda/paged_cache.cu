@@ -98,7 +98,9 @@ struct PrefixPlan {
   bool fast = false;  // the two kernels can address this call; the one-warp-per-row kernel serves the rest
   int dim = 0;        // head dims a kernel is built for: 64 or 128
   int both_rows = 0, row_blocks = 0, tiles = 0, tiles_per_chunk = 0, chunks = 0, records = 0;
-  uint64_t ml_at = 0, total = 0;
+  int tokens_per_item = 1, group_tiles = 1, slot_shift = 0, workers = 0;
+  int64_t slots = 0, fragments = 0;
+  uint64_t ml_at = 0, fragment_o_at = 0, fragment_ml_at = 0, sums_at = 0, total = 0;
 };
 
 PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
@@ -112,29 +114,50 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
            rows_ok(a.q, a.tokens, a.q_stride_token, a.q_heads, a.q_stride_head, 1, 0) && rows_ok(a.out, a.tokens, a.out_stride_token, a.q_heads, a.out_stride_head, 1, 0) &&
            rows_ok(a.k_cache, a.pages, a.k_stride_page, a.page_size, a.k_stride_slot, a.kv_heads, a.k_stride_head) &&
            rows_ok(a.v_cache, a.pages, a.v_stride_page, a.page_size, a.v_stride_slot, a.kv_heads, a.v_stride_head) &&
-           a.tokens * (a.q_heads / a.kv_heads) < (INT64_C(1) << 31) - 256 && a.kv_heads <= 65535;
+           a.tokens * (a.q_heads / a.kv_heads) < (INT64_C(1) << 31) - 256 && a.kv_heads <= 65535 && a.batch < (1 << 24) && a.tokens < (1 << 24);
   if (!p.fast) return p;
   p.dim = a.head_dim <= 64 ? 64 : 128;
-  if (a.prefix_len == 0 || a.tokens == 0 || a.pages == 0) return p;
-  const int64_t rows = a.tokens * (a.q_heads / a.kv_heads);
-  p.both_rows = rows > 128 ? 1 : 0;
-  p.row_blocks = static_cast<int>(p.both_rows ? (rows + 255) / 256 : 1);
-  p.tiles = static_cast<int>((a.prefix_len + 127) / 128);
-  // Cut the prefix so that the waves of work items are full: the cost of a cut is its waves times (tiles of an item + what an
-  // item costs besides, about two tiles: Q, the first loads, the records), and one tile's worth per record written.
-  const int64_t base = a.kv_heads * p.row_blocks;
-  int64_t best = 0;
-  for (int chunks = 1; chunks <= p.tiles && chunks <= 128; ++chunks) {
-    const int per_chunk = (p.tiles + chunks - 1) / chunks;
-    const int used = (p.tiles + per_chunk - 1) / per_chunk;
-    const int64_t waves = (base * used + sms - 1) / sms;
-    const int64_t cost = waves * (per_chunk + 2) * 64 + waves * 32 * (used > 1 ? 1 : 0);
-    if (best == 0 || cost < best) best = cost, p.tiles_per_chunk = per_chunk, p.chunks = used;
+  const int64_t group = a.q_heads / a.kv_heads, rows = a.tokens * group;
+  if (a.prefix_len > 0 && a.tokens > 0 && a.pages > 0) {
+    p.both_rows = rows > 128 ? 1 : 0;
+    p.row_blocks = static_cast<int>(p.both_rows ? (rows + 255) / 256 : 1);
+    p.tiles = static_cast<int>((a.prefix_len + 127) / 128);
+    // Cut the prefix so that the waves of work items are full: the cost of a cut is its waves times (tiles of an item + what an
+    // item costs besides, about two tiles: Q, the first loads, the records), and half a tile's worth per wave for the merge.
+    const int64_t base = a.kv_heads * p.row_blocks;
+    int64_t best = 0;
+    for (int chunks = 1; chunks <= p.tiles && chunks <= 128; ++chunks) {
+      const int per_chunk = (p.tiles + chunks - 1) / chunks;
+      const int used = (p.tiles + per_chunk - 1) / per_chunk;
+      const int64_t waves = (base * used + sms - 1) / sms;
+      const int64_t cost = waves * (per_chunk + 2) * 2 + waves * (used > 1 ? 1 : 0);
+      if (best == 0 || cost < best) best = cost, p.tiles_per_chunk = per_chunk, p.chunks = used;
+    }
+    p.records = p.both_rows ? p.chunks : 2 * p.chunks;
   }
-  p.records = p.both_rows ? p.chunks : 2 * p.chunks;
+  p.tokens_per_item = static_cast<int>(group <= 16 ? 16 / group : 1);
+  p.group_tiles = static_cast<int>((group + 15) / 16);
+  p.slots = a.query_starts == nullptr ? a.batch : a.tokens / p.tokens_per_item + a.batch + 1;
+  while ((p.slots >> p.slot_shift) >= SuffixSdpa<64>::kTableSlots) ++p.slot_shift;
+  // warps for every slice the table could hold, up to what the SMs hold at once
+  const int64_t slices = (a.table_width * a.page_size + 15) / 16, columns = a.kv_heads * p.group_tiles;
+  const int64_t most = static_cast<int64_t>(sms) * SuffixSdpa<64>::kCtasPerSm * SuffixSdpa<64>::kWarps;
+  int64_t wanted = p.slots * columns;
+  wanted = slices == 0 || wanted >= most ? (slices == 0 ? 1 : most) : (wanted * slices < most ? wanted * slices : most);
+  p.workers = static_cast<int>((wanted + 3) / 4 * 4);
+  p.fragments = p.workers + p.slots * columns;
+
+  auto place = [&](uint64_t bytes) {
+    const uint64_t at = p.total;
+    p.total += (bytes + 255) / 256 * 256;
+    return at;
+  };
   const uint64_t record_rows = static_cast<uint64_t>(p.records) * a.kv_heads * rows;
-  p.ml_at = record_rows * p.dim * 4;
-  p.total = p.ml_at + record_rows * 8;
+  place(record_rows * p.dim * 4);
+  p.ml_at = place(record_rows * 8);
+  p.fragment_o_at = place(static_cast<uint64_t>(p.fragments) * 16 * p.dim * 4);
+  p.fragment_ml_at = place(static_cast<uint64_t>(p.fragments) * 16 * 8);
+  p.sums_at = place(static_cast<uint64_t>(p.slots + 1) * 4);
   return p;
 }
 
@@ -143,7 +166,7 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   using G = PrefixTc<kDim>;
   const PrefixSdpaArgs args = prefix_args(a);
   cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
-  cudaLaunchAttribute attributes[2] = {};
+  cudaLaunchAttribute attributes[1] = {};
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
@@ -191,26 +214,31 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   SuffixSdpaArgs s{};
   s.a = args;
   s.rows = rows;
-  s.tokens_per_item = args.group <= 16 ? 16 / args.group : 1;
-  s.group_tiles = (args.group + 15) / 16;
+  s.tokens_per_item = plan.tokens_per_item, s.group_tiles = plan.group_tiles;
+  s.slots = static_cast<int>(plan.slots), s.slot_shift = plan.slot_shift, s.workers = plan.workers;
   s.records = plan.records, s.partial_o = partial_o, s.partial_ml = partial_ml;
-  const int64_t slots = a.query_starts == nullptr ? a.batch : a.tokens / s.tokens_per_item + a.batch + 1;
-  const int64_t items = slots * a.kv_heads * s.group_tiles, capacity = a.table_width * a.page_size;
-  // few items: several CTAs share one, each warp with a slice of sixteen keys at least; two CTAs fit an SM
-  while (s.split_bits < 3 && (items << (s.split_bits + 1)) <= 2 * static_cast<int64_t>(device.sms) && (INT64_C(128) << s.split_bits) <= capacity) ++s.split_bits;
-  if ((slots << s.split_bits) > 0x7fffffff || a.kv_heads * s.group_tiles > 65535)
-    return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
-  s.slots = static_cast<int>(slots);
-  attributes[1].id = cudaLaunchAttributeClusterDimension;
-  attributes[1].val.clusterDim.x = 1u << s.split_bits;
-  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
-  config.gridDim = dim3(static_cast<unsigned>(slots << s.split_bits), static_cast<unsigned>(a.kv_heads * s.group_tiles));
+  char* base = static_cast<char*>(a.workspace);
+  s.fragment_o = reinterpret_cast<float*>(base + plan.fragment_o_at), s.fragment_ml = reinterpret_cast<float2*>(base + plan.fragment_ml_at);
+  s.sums = reinterpret_cast<int*>(base + plan.sums_at);
+  config.gridDim = dim3(static_cast<unsigned>(plan.workers / SuffixSdpa<kDim>::kWarps));
   config.blockDim = dim3(SuffixSdpa<kDim>::kThreads);
   config.dynamicSmemBytes = SuffixSdpa<kDim>::kSmemBytes;
-  config.numAttrs = 2;
-  const cudaError_t status = cudaLaunchKernelEx(&config, suffix_sdpa_kernel<T, kDim>, s);
+  config.numAttrs = 1;
+  cudaError_t status = cudaLaunchKernelEx(&config, suffix_sdpa_kernel<T, kDim>, s);
   if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "suffix_sdpa launch: %s", cudaGetErrorString(status));
-  return decode_launched("suffix_sdpa", error);
+  int32_t rc = decode_launched("suffix_sdpa", error);
+  if (rc != VECOPS_STATUS_OK) return rc;
+  // few rows: four warps share one's partial results
+  const int64_t out_rows = a.tokens * a.q_heads;
+  const bool shared_rows = out_rows <= static_cast<int64_t>(device.sms) * 16;
+  const int64_t blocks = shared_rows ? out_rows : (out_rows + 3) / 4;
+  if (blocks > 0x7fffffff) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(128);
+  config.dynamicSmemBytes = 0;
+  status = shared_rows ? cudaLaunchKernelEx(&config, sdpa_merge_rows_kernel<T, kDim, 4>, s) : cudaLaunchKernelEx(&config, sdpa_merge_rows_kernel<T, kDim, 1>, s);
+  if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "sdpa_merge_rows launch: %s", cudaGetErrorString(status));
+  return decode_launched("sdpa_merge_rows", error);
 }
 
 template <typename T>

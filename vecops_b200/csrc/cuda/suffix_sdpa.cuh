@@ -1,15 +1,15 @@
-// Attention over each sequence's own suffix, merged with what the prefix kernel left: the second half of shared-prefix
-// attention, and all of it when there is no prefix.
+// Attention over each sequence's own suffix, and the merge with what the prefix kernel left: the second and third kernels of
+// shared-prefix attention, and all of it when there is no prefix.
 //
-// A work item is up to sixteen query rows of one sequence and one key/value head - the queries that read this head, of one
-// token or of a few neighbouring ones - against the keys they see.  Its time is the keys' way from memory: every key and
-// value is used by at most sixteen rows.  So the keys go sixteen at a time to the warps of a CTA, and of a cluster of CTAs
-// where there are few items; a warp keeps three such slices in flight for itself by cp.async (no barrier in the
-// loop) and multiplies them with mma.sync m16n8k16, whose sixteen rows are the item's; tcgen05's 128 rows would be nearly
-// empty.  Each warp runs the recurrence m' = max(m, s), l, O of its own slices; at the end the warps of the cluster and
-// the prefix kernel's records meet,
+// An item is up to sixteen query rows of one sequence and one key/value head - the queries that read this head, of one
+// token or of a few neighbouring ones - and the keys they see, in slices of sixteen.  The work is the keys' way from
+// memory: every key and value is used by at most sixteen rows.  So all slices of all items, in order, are dealt out evenly to
+// the warps of the grid whatever the lengths are; a warp keeps the next slice in flight by cp.async while it multiplies
+// one with mma.sync m16n8k16, whose sixteen rows are the item's (tcgen05's 128 would be nearly empty).  Warps share
+// nothing and meet at no barrier.  Each runs m' = max(m, s), l, O over its part of an item and leaves them as a fragment;
+// sdpa_merge_rows_kernel, launched behind, joins a row's fragments and its prefix records,
 //     M = max m_c      out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c           (m in units of log2(e))
-// in an order that does not depend on timing.  Keys that some of the item's rows see and others do not - at most fifteen, the
+// in an order that does not depend on timing.  Keys that some of an item's rows see and others do not - at most fifteen, the
 // newest tokens' own - go past the tensor core: there a zero probability times whatever a later token's value holds
 // would still be NaN.
 #pragma once
@@ -21,18 +21,17 @@ namespace vb200 {
 template <int kDim>
 struct SuffixSdpa {
   static constexpr int kWarps = 4, kThreads = 32 * kWarps;
+  static constexpr int kCtasPerSm = 3;
   static constexpr int kRows = 16, kKeys = 16;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = 2;
   static constexpr int kRowBytes = kDim * 2;
   static constexpr int kTileBytes = kKeys * kRowBytes;
   static constexpr int kWarpBytes = kStages * 2 * kTileBytes;
-  static constexpr int kPitch = kDim + 4;  // floats of a row of O while the warps meet, over the ring
-  static constexpr int kExtraOffset = kWarps * kWarpBytes;
+  static constexpr int kProbOffset = kWarps * kWarpBytes;
   static constexpr int kProbBytes = kRows * kKeys * 4;  // per warp: probabilities of the keys that only some rows see
-  static constexpr int kMlOffset = kExtraOffset + kWarps * kProbBytes;  // [warp][row] (m, l)
-  static constexpr int kSmemBytes = kMlOffset + kWarps * kRows * 8 + kWarps * kStages * 4;
-  static constexpr int kMaxSplit = 8;  // CTAs of a cluster
-  static_assert(kRows * kPitch * 4 <= kWarpBytes, "a warp's O lies over its ring");
+  static constexpr int kTableOffset = kProbOffset + kWarps * kProbBytes;
+  static constexpr int kTableSlots = 1024;              // running sums of the items' slices; more items share an entry
+  static constexpr int kSmemBytes = kTableOffset + (kTableSlots + 1 + kWarps * kStages + 32) * 4;
 };
 
 struct SuffixSdpaArgs {
@@ -40,12 +39,56 @@ struct SuffixSdpaArgs {
   int rows;             // tokens * group, per key/value head: the prefix records' rows
   int tokens_per_item;  // neighbouring tokens of one sequence in an item
   int group_tiles;      // items a token is cut into when its group has more than sixteen heads
-  int slots;            // items per key/value head, idle ones included
-  int split_bits;
-  int records;          // of the prefix kernel; 0: there is none, and nothing to wait for but the kernels before
+  int slots;            // of items per (head, group tile), idle ones included
+  int slot_shift;       // log2 of the slots that share an entry of the table
+  int workers;          // warps of the suffix kernel
+  int records;          // of the prefix kernel
   const float* partial_o;
   const float2* partial_ml;
+  float* fragment_o;    // [warp + item][16][kDim]
+  float2* fragment_ml;  // [warp + item][16]
+  int* sums;            // [slot] slices of the slots before it, written where the slot has any; then [slots] the sum of all
 };
+
+// What a slot holds.  Without query_starts slot b is sequence b's one token; with them sequence b's items are the slots from
+// query_starts[b] / tokens_per_item + b on: apart from each other, and found without a sum.
+struct SuffixItem {
+  int sequence, first, count;  // tokens [first, first + count); count 0: an idle slot
+  int newest, length;
+};
+
+__device__ __forceinline__ int suffix_sees(const PrefixSdpaArgs& a, int length, int newest, int t) {
+  const long long capacity = static_cast<long long>(a.table_width) * a.page_size;
+  const long long seen = static_cast<long long>(length) - (newest - t);
+  return static_cast<int>(seen < 0 ? 0 : seen < capacity ? seen : capacity);
+}
+
+// The last sequence whose query_starts pass `before`, by a search 32 wide; the whole warp comes here.
+template <typename Before>
+__device__ __forceinline__ int suffix_search(int batch, const Before& before) {
+  const int lane = threadIdx.x & 31;
+  int low = 0, high = batch;
+  while (high - low > 1) {
+    const int step = (high - low + 31) / 32, probe = low + lane * step;
+    const int found = 31 - __clz(__ballot_sync(0xffffffffu, probe < high && before(probe)) | 1u);
+    low += found * step;
+    high = min(high, low + step);
+  }
+  return low;
+}
+
+__device__ __forceinline__ SuffixItem suffix_item(const SuffixSdpaArgs& p, int slot) {
+  SuffixItem item{slot, slot, 1, slot, -1};
+  if (p.a.query_starts != nullptr) {
+    item.sequence = suffix_search(p.a.batch, [&](int b) { return p.a.query_starts[b] / p.tokens_per_item + b <= slot; });
+    const int start = p.a.query_starts[item.sequence], end = p.a.query_starts[item.sequence + 1];
+    item.first = start + (slot - (start / p.tokens_per_item + item.sequence)) * p.tokens_per_item;
+    item.count = min(p.tokens_per_item, end - item.first);
+    item.newest = end - 1;
+  }
+  item.length = p.a.lengths[item.sequence];
+  return item;
+}
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -89,321 +132,395 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) {
 }
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, 2) suffix_sdpa_kernel(const SuffixSdpaArgs p) {
+__global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::kCtasPerSm) suffix_sdpa_kernel(const SuffixSdpaArgs p) {
   using G = SuffixSdpa<kDim>;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t smem_base = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = 1 << p.split_bits, part = static_cast<int>(blockIdx.x) & (split - 1);
-  const int kv = static_cast<int>(blockIdx.y) / p.group_tiles, group0 = static_cast<int>(blockIdx.y) % p.group_tiles * 16;
-  const int slot = static_cast<int>(blockIdx.x) >> p.split_bits;
   const PrefixSdpaArgs& a = p.a;
+  int* table = reinterpret_cast<int*>(smem + G::kTableOffset);  // [entry] slices of the slots before the entry's
+  volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(table + G::kTableSlots + 1) + warp * G::kStages;
+  int* warp_sums = table + G::kTableSlots + 1 + G::kWarps * G::kStages;
   if (p.records == 0) grid_dependency_wait();  // (with a prefix kernel in between, the kernels before that one are done already)
+  grid_launch_dependents();
 
-  // ---------------------------------------------------------------- which sequence, which of its tokens
-  // Sequence b's items are the slots from query_starts[b] / tokens_per_item + b on: apart from each other, and found without a sum.
-  int sequence = slot, first = slot, count = 1, begin_all = 0, end_all = a.tokens;
-  bool idle = slot >= p.slots || slot >= a.batch;
-  if (a.query_starts != nullptr) {
-    idle = slot >= p.slots - 1 || a.batch == 0;
-    begin_all = a.query_starts[0], end_all = a.query_starts[a.batch];
-    int low = 0, high = a.batch;  // the last b whose slots start at or before this one
-    while (high - low > 1) {
-      const int step = (high - low + 31) / 32;
-      const int probe = low + lane * step;
-      const bool before = probe < high && a.query_starts[probe] / p.tokens_per_item + probe <= slot;
-      const int found = 31 - __clz(__ballot_sync(0xffffffffu, before) | 1u);
-      low += found * step;
-      high = min(high, low + step);
-    }
-    if (!idle) {
-      sequence = low;
-      const int start = a.query_starts[low], tile = slot - (start / p.tokens_per_item + low);
-      first = start + tile * p.tokens_per_item;
-      count = min(p.tokens_per_item, a.query_starts[low + 1] - first);
-      idle = tile < 0 || first < 0 || count <= 0 || first + count > a.tokens;
+  // ---------------------------------------------------------------- how many slices come before each slot
+  const int entries = (p.slots + (1 << p.slot_shift) - 1) >> p.slot_shift;
+  for (int e = threadIdx.x; e < G::kTableSlots + 1; e += G::kThreads) table[e] = 0;
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.batch; b += G::kThreads) {
+    const int length = a.lengths[b];
+    if (length <= 0) continue;
+    if (a.query_starts == nullptr) {
+      atomicAdd(table + (b >> p.slot_shift), (suffix_sees(a, length, b, b) + G::kKeys - 1) / G::kKeys);
+    } else {
+      const int start = max(0, a.query_starts[b]), end = min(a.tokens, a.query_starts[b + 1]);
+      int slot = start / p.tokens_per_item + b;
+      for (int first = start; first < end && slot < p.slots; first += p.tokens_per_item, ++slot)
+        atomicAdd(table + (slot >> p.slot_shift), (suffix_sees(a, length, end - 1, min(end, first + p.tokens_per_item) - 1) + G::kKeys - 1) / G::kKeys);
     }
   }
-  if (slot == p.slots - 1 && a.query_starts != nullptr && part == 0 && group0 == 0) {
-    // the spare last slot zeroes the tokens of no sequence
-    for (int t = warp; t < a.tokens; t += G::kWarps) {
-      if (t >= begin_all && t < end_all) continue;
-      for (int i = lane; i < a.group * a.head_dim; i += 32)
-        (static_cast<T*>(a.out) + t * a.o_st + (kv * a.group + i / a.head_dim) * a.o_sh)[i % a.head_dim] = append_down<T>(0.f);
-    }
-  }
-  if (idle) return;  // (uniform over the cluster, whose CTAs share the slot)
-  const int length = a.lengths[sequence];
-  const int heads = min(16, a.group - group0);  // rows are [token][head in group]
-  const int rows = count * heads;
-  if (length < 0) {
-    if (part == 0) {
-      for (int i = threadIdx.x; i < rows * a.head_dim; i += G::kThreads) {
-        const int r = i / a.head_dim, t = first + r / heads, head = kv * a.group + group0 + r % heads;
-        (static_cast<T*>(a.out) + t * a.o_st + head * a.o_sh)[i % a.head_dim] = append_down<T>(0.f);
-      }
-    }
-    return;
-  }
-  // suffix keys the item's first and last token see
-  const int newest = a.query_starts != nullptr ? a.query_starts[sequence + 1] - 1 : first;
-  const long long capacity = static_cast<long long>(a.table_width) * a.page_size;
-  auto sees_of = [&](int t) {
-    const long long seen = static_cast<long long>(length) - (newest - t);
-    return static_cast<int>(seen < 0 ? 0 : seen < capacity ? seen : capacity);
-  };
-  const int all_see = sees_of(first), some_see = sees_of(first + count - 1);
-
-  // ---------------------------------------------------------------- this warp's slices: worker, worker + workers, ...
-  const int workers = G::kWarps << p.split_bits, worker = part * G::kWarps + warp;
-  const int slices = (some_see + G::kKeys - 1) / G::kKeys;
-  const int mine = slices > worker ? (slices - worker + workers - 1) / workers : 0;
-  const uint32_t ring = smem_base + warp * G::kWarpBytes;
-  volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(smem + G::kMlOffset + G::kWarps * G::kRows * 8) + warp * G::kStages;
-  const T* k_base = static_cast<const T*>(a.k) + kv * a.k_sh;
-  const T* v_base = static_cast<const T*>(a.v) + kv * a.v_sh;
-  const int* table = a.page_table + sequence * a.table_stride;
-  auto page_of = [&](int i) {  // page of this lane's key (lanes 0..15) in slice i, or -1
-    const int key = (worker + i * workers) * G::kKeys + (lane & 15);
-    return i < mine && key < some_see ? __ldg(table + key / a.page_size) : -1;
-  };
-  constexpr int kPieces = kDim / 8;                   // 16-byte pieces of a row
-  constexpr int kRowsPerStep = 32 / kPieces;          // rows a warp-wide copy covers
-  int page_next = page_of(0);
-  auto issue = [&](int i) {
-    const int stage = i % G::kStages;
-    const int page = page_next;
-    page_next = page_of(i + 1);
-    if (i < mine) {
-      const int key = (worker + i * workers) * G::kKeys + (lane & 15);
-      const bool there = page >= 0 && page < a.pages;
-      const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
-      if (lane == 0) present[stage] = mask;
-      const long long offset = key % a.page_size;
-      const long long k_at = there ? page * a.k_sp + offset * a.k_ss : 0, v_at = there ? page * a.v_sp + offset * a.v_ss : 0;
-      const uint32_t dst = ring + stage * 2 * G::kTileBytes;
-      const int piece = lane % kPieces;
-#pragma unroll
-      for (int step = 0; step < G::kKeys / kRowsPerStep; ++step) {
-        const int row = step * kRowsPerStep + lane / kPieces;
-        const long long k_row = __shfl_sync(0xffffffffu, k_at, row), v_row = __shfl_sync(0xffffffffu, v_at, row);
-        const uint32_t bytes = (mask >> row & 1u) != 0 && piece * 8 < a.head_dim ? 16 : 0;
-        const uint32_t to = dst + row * G::kRowBytes + ((piece ^ (row & 7)) << 4);
-        cp_async_16(to, k_base + k_row + (bytes != 0 ? piece * 8 : 0), bytes);
-        cp_async_16(to + G::kTileBytes, v_base + v_row + (bytes != 0 ? piece * 8 : 0), bytes);
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < G::kStages - 1; ++i) issue(i);
-
-  // Q: the A fragments of sixteen rows
-  const int r_low = lane >> 2, r_high = r_low + 8;
-  uint32_t q[kDim / 16][4];
+  __syncthreads();
   {
-    const T* q_row[2];
-    bool there[2];
+    // exclusive sums over the entries, eight a thread
+    constexpr int kMine = G::kTableSlots / G::kThreads;
+    int mine[kMine], sum = 0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = h == 0 ? r_low : r_high;
-      there[h] = r < rows;
-      const int t = first + (there[h] ? r / heads : 0), head = kv * a.group + group0 + (there[h] ? r % heads : 0);
-      q_row[h] = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
+    for (int e = 0; e < kMine; ++e) mine[e] = table[threadIdx.x * kMine + e], sum += mine[e];
+    int before = sum;
+#pragma unroll
+    for (int offset = 1; offset < 32; offset <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, before, offset);
+      if (lane >= offset) before += other;
     }
+    if (lane == 31) warp_sums[warp] = before;
+    __syncthreads();
+    before -= sum;
+    for (int w = 0; w < warp; ++w) before += warp_sums[w];
 #pragma unroll
-    for (int ks = 0; ks < kDim / 16; ++ks)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = ks * 16 + (lane & 3) * 2 + (e >> 1) * 8;
-        q[ks][e] = there[e & 1] && d < a.head_dim ? *reinterpret_cast<const uint32_t*>(q_row[e & 1] + d) : 0u;
-      }
+    for (int e = 0; e < kMine; ++e) table[threadIdx.x * kMine + e] = before, before += mine[e];
+    if (threadIdx.x == G::kThreads - 1) table[G::kTableSlots] = before;
+    __syncthreads();
   }
-  const int sees[2] = {r_low < rows ? sees_of(first + r_low / heads) : 0, r_high < rows ? sees_of(first + r_high / heads) : 0};
-  const float scale = a.scale * 1.4426950408889634f;
-  float o[kDim / 8][4];
-#pragma unroll
-  for (int nt = 0; nt < kDim / 8; ++nt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float* probabilities = reinterpret_cast<float*>(smem + G::kExtraOffset + warp * G::kProbBytes);
+  const int columns = a.kv_heads * p.group_tiles;  // items of a slot
+  const long long all = static_cast<long long>(table[G::kTableSlots]) * columns;
+  const int worker = static_cast<int>(blockIdx.x) * G::kWarps + warp;
+  if (worker == 0 && lane == 0) p.sums[p.slots] = table[G::kTableSlots];
 
-  for (int i = 0; i < mine; ++i) {
-    issue(i + G::kStages - 1);
-    cp_async_wait<G::kStages - 1>();
-    __syncwarp();
-    const int stage = i % G::kStages, key0 = (worker + i * workers) * G::kKeys;
-    const uint32_t k_tile = ring + stage * 2 * G::kTileBytes, v_tile = k_tile + G::kTileBytes;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-    for (int ks = 0; ks < kDim / 16; ++ks) {
-      const int key = (lane >> 4) * 8 + (lane & 7), piece = ks * 2 + ((lane >> 3) & 1);
-      uint32_t b[4];
-      ldmatrix_x4(b, k_tile + key * G::kRowBytes + ((piece ^ (key & 7)) << 4));
-      mma_16816<T>(s[0], q[ks], b[0], b[1]);
-      mma_16816<T>(s[1], q[ks], b[2], b[3]);
+  // ---------------------------------------------------------------- this warp's slices [position, end)
+  const long long workers = min(static_cast<long long>(p.workers), all);  // (no warp is dealt nothing while another has something)
+  long long position = worker < workers ? all * worker / workers : 0;
+  const long long end = worker < workers ? all * (worker + 1) / workers : 0;
+  const uint32_t ring = smem_base + warp * G::kWarpBytes;
+  float* probabilities = reinterpret_cast<float*>(smem + G::kProbOffset + warp * G::kProbBytes);
+  while (position < end) {
+    // the slot: by the table, and where several share an entry by counting on from its first
+    const int before_slot = static_cast<int>(position / columns);  // (a slot's items have the same number of slices)
+    int low = 0, high = entries;
+    while (high - low > 1) {
+      const int middle = (low + high) / 2;
+      if (table[middle] <= before_slot) low = middle;
+      else high = middle;
     }
-    const uint32_t mask = present[stage];
-    float top[2] = {-INFINITY, -INFINITY};
+    int slot = low << p.slot_shift, slot_sum = table[low], slices = 0;
+    SuffixItem item;
+    for (;; ++slot) {
+      item = suffix_item(p, slot);
+      const bool idle = item.count <= 0 || item.first < 0 || item.first + item.count > a.tokens || item.length <= 0 ||
+                        (a.query_starts != nullptr && item.first < a.query_starts[item.sequence]);
+      slices = idle ? 0 : (suffix_sees(a, item.length, item.newest, item.first + item.count - 1) + G::kKeys - 1) / G::kKeys;
+      if (before_slot < slot_sum + slices || slot + 1 >= p.slots) break;
+      slot_sum += slices;
+    }
+    if (slices <= 0) break;  // (the table and this count agree: not reached)
+    if (lane == 0) p.sums[slot] = slot_sum;
+    const long long in_slot = position - static_cast<long long>(slot_sum) * columns;
+    const int column = static_cast<int>(in_slot / slices), first_slice = static_cast<int>(in_slot - static_cast<long long>(column) * slices);
+    const int mine = static_cast<int>(min(static_cast<long long>(slices - first_slice), end - position));
+    position += mine;
+    const int kv = column / p.group_tiles, group0 = column % p.group_tiles * 16;
+    const int heads = min(16, a.group - group0), rows = item.count * heads;  // rows are [token][head in group]
+    const int first = item.first;
+    auto sees_of = [&](int t) { return suffix_sees(a, item.length, item.newest, t); };
+    const int all_see = sees_of(first), some_see = sees_of(first + item.count - 1);
+
+    const T* k_base = static_cast<const T*>(a.k) + kv * a.k_sh;
+    const T* v_base = static_cast<const T*>(a.v) + kv * a.v_sh;
+    const int* pages = a.page_table + item.sequence * a.table_stride;
+    auto page_of = [&](int i) {  // page of this lane's key (lanes 0..15) in slice i, or -1
+      const int key = (first_slice + i) * G::kKeys + (lane & 15);
+      return i < mine && key < some_see ? __ldg(pages + key / a.page_size) : -1;
+    };
+    constexpr int kPieces = kDim / 8;           // 16-byte pieces of a row
+    constexpr int kRowsPerStep = 32 / kPieces;  // rows a warp-wide copy covers
+    int page_next = page_of(0), page_after = page_of(1);
+    auto issue = [&](int i) {
+      const int stage = i % G::kStages;
+      const int page = page_next;
+      page_next = page_after;
+      page_after = page_of(i + 2);
+      if (i < mine) {
+        const int key = (first_slice + i) * G::kKeys + (lane & 15);
+        const bool there = page >= 0 && page < a.pages;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
+        if (lane == 0) present[stage] = mask;
+        const long long offset = key % a.page_size;
+        const long long k_at = there ? page * a.k_sp + offset * a.k_ss : 0, v_at = there ? page * a.v_sp + offset * a.v_ss : 0;
+        const uint32_t dst = ring + stage * 2 * G::kTileBytes;
+        const int piece = lane % kPieces;
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = nt * 8 + (lane & 3) * 2 + (e & 1);
-        const bool keep = key0 + key < sees[e >> 1] && (mask >> key & 1u) != 0;
-        s[nt][e] = keep ? s[nt][e] * scale : -INFINITY;
-        top[e >> 1] = fmaxf(top[e >> 1], s[nt][e]);
+        for (int step = 0; step < G::kKeys / kRowsPerStep; ++step) {
+          const int row = step * kRowsPerStep + lane / kPieces;
+          const long long k_row = __shfl_sync(0xffffffffu, k_at, row), v_row = __shfl_sync(0xffffffffu, v_at, row);
+          const uint32_t bytes = (mask >> row & 1u) != 0 && piece * 8 < a.head_dim ? 16 : 0;
+          const uint32_t to = dst + row * G::kRowBytes + ((piece ^ (row & 7)) << 4);
+          cp_async_16(to, k_base + k_row + (bytes != 0 ? piece * 8 : 0), bytes);
+          cp_async_16(to + G::kTileBytes, v_base + v_row + (bytes != 0 ? piece * 8 : 0), bytes);
+        }
       }
-    bool moves = false;
-    float m_new[2];
+      cp_async_commit();
+    };
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      // the maximum is moved only when it would grow by more than 2^8: O and l carry the same one, so nothing is lost
-      m_new[h] = top[h] > m[h] + 8.f ? top[h] : m[h];
-      moves = moves || m_new[h] != m[h];
-    }
-    if (__any_sync(0xffffffffu, moves)) {
+    for (int i = 0; i < G::kStages - 1; ++i) issue(i);
+
+    // Q: the A fragments of sixteen rows
+    const int r_low = lane >> 2, r_high = r_low + 8;
+    uint32_t q[kDim / 16][4];
+    {
+      const T* q_row[2];
+      bool there[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float keep = m_new[h] == m[h] ? 1.f : exp2_approx(m[h] - m_new[h]);
-        m[h] = m_new[h];
-        l[h] *= keep;
-#pragma unroll
-        for (int nt = 0; nt < kDim / 8; ++nt) o[nt][2 * h] *= keep, o[nt][2 * h + 1] *= keep;
+        const int r = h == 0 ? r_low : r_high;
+        there[h] = r < rows;
+        const int t = first + (there[h] ? r / heads : 0), head = kv * a.group + group0 + (there[h] ? r % heads : 0);
+        q_row[h] = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
       }
+#pragma unroll
+      for (int ks = 0; ks < kDim / 16; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = ks * 16 + (lane & 3) * 2 + (e >> 1) * 8;
+          q[ks][e] = there[e & 1] && d < a.head_dim ? *reinterpret_cast<const uint32_t*>(q_row[e & 1] + d) : 0u;
+        }
     }
+    const int sees[2] = {r_low < rows ? sees_of(first + r_low / heads) : 0, r_high < rows ? sees_of(first + r_high / heads) : 0};
+    const float scale = a.scale * 1.4426950408889634f;
+    float o[kDim / 8][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
+    for (int nt = 0; nt < kDim / 8; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float base = m[e >> 1] == -INFINITY ? 0.f : m[e >> 1];
-        s[nt][e] = exp2_approx(s[nt][e] - base);
-        l[e >> 1] += s[nt][e];
-      }
-    if (key0 + G::kKeys > all_see && all_see < some_see) {
-      // keys that not every row sees: added here, one by one, where a row that does not see a key does not touch its value
+      for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int i = 0; i < mine; ++i) {
+      issue(i + G::kStages - 1);
+      cp_async_wait<G::kStages - 1>();
       __syncwarp();
+      const int stage = i % G::kStages, key0 = (first_slice + i) * G::kKeys;
+      const uint32_t k_tile = ring + stage * 2 * G::kTileBytes, v_tile = k_tile + G::kTileBytes;
+      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int ks = 0; ks < kDim / 16; ++ks) {
+        const int key = (lane >> 4) * 8 + (lane & 7), piece = ks * 2 + ((lane >> 3) & 1);
+        uint32_t b[4];
+        ldmatrix_x4(b, k_tile + key * G::kRowBytes + ((piece ^ (key & 7)) << 4));
+        mma_16816<T>(s[0], q[ks], b[0], b[1]);
+        mma_16816<T>(s[1], q[ks], b[2], b[3]);
+      }
+      const uint32_t mask = present[stage];
+      float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = nt * 8 + (lane & 3) * 2 + (e & 1);
-          probabilities[(e < 2 ? r_low : r_high) * G::kKeys + key] = s[nt][e];
-          if (key0 + key >= all_see) s[nt][e] = 0.f;
+          const bool keep = key0 + key < sees[e >> 1] && (mask >> key & 1u) != 0;
+          s[nt][e] = keep ? s[nt][e] * scale : -INFINITY;
+          top[e >> 1] = fmaxf(top[e >> 1], s[nt][e]);
         }
-      __syncwarp();
+      bool moves = false;
+      float m_new[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+        // the maximum is moved only when it would grow by more than 2^8: O and l carry the same one, so nothing is lost
+        m_new[h] = top[h] > m[h] + 8.f ? top[h] : m[h];
+        moves = moves || m_new[h] != m[h];
+      }
+      if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float keep = m_new[h] == m[h] ? 1.f : exp2_approx(m[h] - m_new[h]);
+          m[h] = m_new[h];
+          l[h] *= keep;
+#pragma unroll
+          for (int nt = 0; nt < kDim / 8; ++nt) o[nt][2 * h] *= keep, o[nt][2 * h + 1] *= keep;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float base = m[e >> 1] == -INFINITY ? 0.f : m[e >> 1];
+          s[nt][e] = exp2_approx(s[nt][e] - base);
+          l[e >> 1] += s[nt][e];
+        }
+      if (key0 + G::kKeys > all_see && all_see < some_see) {
+        // keys that not every row sees: added here, one by one, where a row that does not see a key does not touch its value
+        __syncwarp();
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = nt * 8 + (lane & 3) * 2 + (e & 1);
+            probabilities[(e < 2 ? r_low : r_high) * G::kKeys + key] = s[nt][e];
+            if (key0 + key >= all_see) s[nt][e] = 0.f;
+          }
+        __syncwarp();
 #pragma unroll 1
-      for (int key = max(0, all_see - key0); key < min(G::kKeys, some_see - key0); ++key) {
-        const float p_low = probabilities[r_low * G::kKeys + key], p_high = probabilities[r_high * G::kKeys + key];
+        for (int key = max(0, all_see - key0); key < min(G::kKeys, some_see - key0); ++key) {
+          const float p_low = probabilities[r_low * G::kKeys + key], p_high = probabilities[r_high * G::kKeys + key];
 #pragma unroll
-        for (int nt = 0; nt < kDim / 8; ++nt) {
-          uint32_t raw;
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(raw) : "r"(v_tile + key * G::kRowBytes + ((nt ^ (key & 7)) << 4) + (lane & 3) * 4) : "memory");
-          const float2 x = unpack2<T>(raw);
-          if (p_low != 0.f) o[nt][0] = fmaf(p_low, x.x, o[nt][0]), o[nt][1] = fmaf(p_low, x.y, o[nt][1]);
-          if (p_high != 0.f) o[nt][2] = fmaf(p_high, x.x, o[nt][2]), o[nt][3] = fmaf(p_high, x.y, o[nt][3]);
+          for (int nt = 0; nt < kDim / 8; ++nt) {
+            uint32_t raw;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(raw) : "r"(v_tile + key * G::kRowBytes + ((nt ^ (key & 7)) << 4) + (lane & 3) * 4) : "memory");
+            const float2 x = unpack2<T>(raw);
+            if (p_low != 0.f) o[nt][0] = fmaf(p_low, x.x, o[nt][0]), o[nt][1] = fmaf(p_low, x.y, o[nt][1]);
+            if (p_high != 0.f) o[nt][2] = fmaf(p_high, x.x, o[nt][2]), o[nt][3] = fmaf(p_high, x.y, o[nt][3]);
+          }
         }
+        __syncwarp();
+        for (int piece = lane; piece < G::kKeys * kPieces; piece += 32) {
+          const int key = piece / kPieces;
+          if (key0 + key >= all_see)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_tile + key * G::kRowBytes + (piece % kPieces << 4)), "r"(0) : "memory");
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      for (int piece = lane; piece < G::kKeys * kPieces; piece += 32) {
-        const int key = piece / kPieces;
-        if (key0 + key >= all_see)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_tile + key * G::kRowBytes + (piece % kPieces << 4)), "r"(0) : "memory");
+      const uint32_t pa[4] = {prefix_pack<T>(s[0][0], s[0][1]), prefix_pack<T>(s[0][2], s[0][3]), prefix_pack<T>(s[1][0], s[1][1]),
+                              prefix_pack<T>(s[1][2], s[1][3])};
+#pragma unroll
+      for (int nt = 0; nt < kDim / 8; nt += 2) {
+        const int key = ((lane >> 3) & 1) * 8 + (lane & 7), piece = nt + (lane >> 4);
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, v_tile + key * G::kRowBytes + ((piece ^ (key & 7)) << 4));
+        mma_16816<T>(o[nt], pa, b[0], b[1]);
+        mma_16816<T>(o[nt + 1], pa, b[2], b[3]);
       }
-      __syncwarp();
+      __syncwarp();  // the slice has been read by every lane before its stage is filled again
     }
-    const uint32_t pa[4] = {prefix_pack<T>(s[0][0], s[0][1]), prefix_pack<T>(s[0][2], s[0][3]), prefix_pack<T>(s[1][0], s[1][1]),
-                            prefix_pack<T>(s[1][2], s[1][3])};
-#pragma unroll
-    for (int nt = 0; nt < kDim / 8; nt += 2) {
-      const int key = ((lane >> 3) & 1) * 8 + (lane & 7), piece = nt + (lane >> 4);
-      uint32_t b[4];
-      ldmatrix_x4_trans(b, v_tile + key * G::kRowBytes + ((piece ^ (key & 7)) << 4));
-      mma_16816<T>(o[nt], pa, b[0], b[1]);
-      mma_16816<T>(o[nt + 1], pa, b[2], b[3]);
-    }
-    __syncwarp();  // the slice has been read by every lane before its stage is filled again
-  }
-  cp_async_wait<0>();
-  __syncwarp();
+    cp_async_wait<0>();
+    __syncwarp();
 
-  // ---------------------------------------------------------------- the warps leave (O, m, l) in shared memory
-  float* mine_o = reinterpret_cast<float*>(smem + warp * G::kWarpBytes);
-  float2* mine_ml = reinterpret_cast<float2*>(smem + G::kMlOffset) + warp * G::kRows;
+    // ---- the fragment leaves
+    const size_t at = (static_cast<size_t>(worker) + static_cast<size_t>(slot) * columns + column) * G::kRows;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if ((lane & 3) == 0) mine_ml[h == 0 ? r_low : r_high] = make_float2(m[h], l[h]);
+    for (int h = 0; h < 2; ++h) {
+      const int r = h == 0 ? r_low : r_high;
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (r < rows) {
+        if ((lane & 3) == 0) __stcg(p.fragment_ml + at + r, make_float2(m[h], l[h]));
 #pragma unroll
-    for (int nt = 0; nt < kDim / 8; ++nt)
-      *reinterpret_cast<float2*>(mine_o + (h == 0 ? r_low : r_high) * G::kPitch + nt * 8 + (lane & 3) * 2) = make_float2(o[nt][2 * h], o[nt][2 * h + 1]);
-  }
-  __syncthreads();
-  if (split > 1) cluster_sync_all();
-  if (p.records > 0) grid_dependency_wait();  // the prefix kernel's records
-
-  // ---------------------------------------------------------------- and meet: a warp per row, four dims a lane
-  for (int r = part + (warp << p.split_bits); r < rows; r += G::kWarps << p.split_bits) {
-    const int t = first + r / heads, in_group = group0 + r % heads;
-    // lane c holds (m, l) of partial c: the warps of the cluster first, then the records of the prefix, 32 at a time
-    const uint32_t ml_at = smem_base + G::kMlOffset + ((lane & (G::kWarps - 1)) * G::kRows + r) * 8;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < workers) {
-      const uint32_t from = map_to_cta(ml_at, lane / G::kWarps);
-      ml = make_float2(ld_shared_cluster_f32(from), ld_shared_cluster_f32(from + 4));
+        for (int nt = 0; nt < kDim / 8; ++nt)
+          __stcg(reinterpret_cast<float2*>(p.fragment_o + (at + r) * kDim + nt * 8 + (lane & 3) * 2), make_float2(o[nt][2 * h], o[nt][2 * h + 1]));
+      }
     }
-    const size_t record_row = static_cast<size_t>(kv) * p.rows + static_cast<size_t>(t) * a.group + in_group;
-    const size_t record_step = static_cast<size_t>(a.kv_heads) * p.rows;
+  }
+  grid_dependency_wait();  // this kernel is done when the prefix kernel is, too: the merge waits for this one alone
+}
+
+// The merge: kRowWarps warps per query row, each with its share of the row's partial results.
+template <typename T, int kDim, int kRowWarps>
+__global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaArgs p) {
+  const PrefixSdpaArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = warp % kRowWarps;
+  const long long index = static_cast<long long>(blockIdx.x) * (4 / kRowWarps) + warp / kRowWarps;  // row: token, query head
+  const bool there = index < static_cast<long long>(a.tokens) * a.q_heads;
+  const int t = there ? static_cast<int>(index / a.q_heads) : 0, head = there ? static_cast<int>(index - static_cast<long long>(t) * a.q_heads) : 0;
+  const int kv = head / a.group, in_group = head - kv * a.group;
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  // the row's sequence, item and fragments
+  int sequence = t, start = t, newest = t;
+  bool owned = there;
+  if (a.query_starts != nullptr) {
+    owned = there && a.batch > 0 && t >= a.query_starts[0] && t < a.query_starts[a.batch];
+    sequence = owned ? suffix_search(a.batch, [&](int b) { return a.query_starts[b] <= t; }) : 0;  // (the same for the warp)
+    if (owned) start = a.query_starts[sequence], newest = a.query_starts[sequence + 1] - 1;
+  }
+  const int length = owned ? a.lengths[sequence] : -1;
+  owned = owned && length >= 0;
+  int fragments = 0;
+  size_t first_fragment = 0;  // its row in the fragments
+  if (owned && length > 0) {
+    const int tile = (t - start) / p.tokens_per_item, first = start + tile * p.tokens_per_item;
+    const int slot = a.query_starts != nullptr ? start / p.tokens_per_item + sequence + tile : sequence;
+    const int last = min(newest, first + p.tokens_per_item - 1);
+    const int slices = (suffix_sees(a, length, newest, last) + 15) / 16;
+    if (slices > 0) {
+      const int columns = a.kv_heads * p.group_tiles, column = kv * p.group_tiles + in_group / 16;
+      const long long all = static_cast<long long>(__ldcg(p.sums + p.slots)) * columns;
+      const long long from = static_cast<long long>(__ldcg(p.sums + slot)) * columns + static_cast<long long>(column) * slices;
+      const long long workers = min(static_cast<long long>(p.workers), all);
+      auto worker_of = [&](long long slice) { return ((slice + 1) * workers - 1) / all; };  // whose [all w / workers, all (w + 1) / workers) has it
+      const long long first_worker = worker_of(from);
+      fragments = static_cast<int>(worker_of(from + slices - 1) - first_worker) + 1;
+      const int heads = min(16, a.group - in_group / 16 * 16);
+      first_fragment = (static_cast<size_t>(first_worker) + static_cast<size_t>(slot) * columns + column) * 16 + (t - first) * heads + in_group % 16;
+    }
+  }
+  const size_t record_row = static_cast<size_t>(kv) * p.rows + static_cast<size_t>(t) * a.group + in_group;
+  const size_t record_step = static_cast<size_t>(a.kv_heads) * p.rows;
+  const int sources = owned ? fragments + p.records : 0;
+  auto ml_of = [&](int c) {
+    return c < fragments ? __ldcg(p.fragment_ml + first_fragment + static_cast<size_t>(c) * 16) : __ldcg(p.partial_ml + (c - fragments) * record_step + record_row);
+  };
+  auto o_of = [&](int c) {
+    return c < fragments ? p.fragment_o + (first_fragment + static_cast<size_t>(c) * 16) * kDim : p.partial_o + ((c - fragments) * record_step + record_row) * kDim;
+  };
+
+  // ---- this warp's share: a block of sources at a time, a lane per (m, l), four dims a lane
+  constexpr int kBlock = kRowWarps > 1 ? 8 : 32;
+  const bool active = lane * 4 < kDim;
+  float m = -INFINITY, l = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = part * kBlock; c0 < sources; c0 += kRowWarps * kBlock) {
+    const int here = min(kBlock, sources - c0);
+    const float2 ml = lane < here ? ml_of(c0 + lane) : make_float2(-INFINITY, 0.f);
     float highest = ml.x;
-    for (int c = lane; c < p.records; c += 32) highest = fmaxf(highest, __ldcg(p.partial_ml + c * record_step + record_row).x);
 #pragma unroll
     for (int offset = 16; offset > 0; offset >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, offset));
-    float weight = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - highest);
-    float total = weight * ml.y;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool active = lane * 4 < kDim;
-    for (int c = 0; c < workers; ++c) {
-      const float w = __shfl_sync(0xffffffffu, weight, c);
-      if (w == 0.f || !active) continue;
-      const float4 x = ld_shared_cluster_v4(map_to_cta(smem_base + (c & (G::kWarps - 1)) * G::kWarpBytes + (r * G::kPitch + lane * 4) * 4, c / G::kWarps));
-      sum.x = fmaf(w, x.x, sum.x), sum.y = fmaf(w, x.y, sum.y), sum.z = fmaf(w, x.z, sum.z), sum.w = fmaf(w, x.w, sum.w);
-    }
-    for (int c0 = 0; c0 < p.records; c0 += 32) {
-      float2 record = make_float2(-INFINITY, 0.f);
-      if (c0 + lane < p.records) record = __ldcg(p.partial_ml + (c0 + lane) * record_step + record_row);
-      weight = record.x == -INFINITY ? 0.f : exp2_approx(record.x - highest);
-      total += weight * record.y;
-      const int here = min(32, p.records - c0);
-      for (int c = 0; c < here; c += 8) {
-        float4 x[8];
+    if (highest == -INFINITY) continue;
+    const float m_new = fmaxf(m, highest), keep = m == -INFINITY ? 0.f : exp2_approx(m - m_new);
+    m = m_new;
+    const float weight = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - m);
+    l = l * keep + weight * ml.y;
+    sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
+    for (int c = 0; c < here; c += 8) {
+      float4 x[8];
+      float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float w = __shfl_sync(0xffffffffu, weight, (c + e) & 31);
-          x[e] = c + e < here && w != 0.f && active ? __ldcg(reinterpret_cast<const float4*>(p.partial_o + ((c0 + c + e) * record_step + record_row) * kDim) + lane)
-                                                    : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float w = c + e < here ? __shfl_sync(0xffffffffu, weight, (c + e) & 31) : 0.f;
-          if (w != 0.f) sum.x = fmaf(w, x[e].x, sum.x), sum.y = fmaf(w, x[e].y, sum.y), sum.z = fmaf(w, x[e].z, sum.z), sum.w = fmaf(w, x[e].w, sum.w);
-        }
+      for (int e = 0; e < 8; ++e) {
+        w[e] = __shfl_sync(0xffffffffu, weight, (c + e) & 31);  // (0 past the last)
+        x[e] = w[e] != 0.f && active ? __ldcg(reinterpret_cast<const float4*>(o_of(c0 + c + e)) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-    }
 #pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) total += __shfl_xor_sync(0xffffffffu, total, offset);
-    const float reciprocal = total == 0.f ? 0.f : 1.f / total;  // no key: zeros
-    if (active && lane * 4 < a.head_dim) {
-      T* out = static_cast<T*>(a.out) + t * a.o_st + (kv * a.group + in_group) * a.o_sh + lane * 4;
-      *reinterpret_cast<uint2*>(out) = make_uint2(prefix_pack<T>(sum.x * reciprocal, sum.y * reciprocal), prefix_pack<T>(sum.z * reciprocal, sum.w * reciprocal));
+      for (int e = 0; e < 8; ++e) sum.x = fmaf(w[e], x[e].x, sum.x), sum.y = fmaf(w[e], x[e].y, sum.y), sum.z = fmaf(w[e], x[e].z, sum.z), sum.w = fmaf(w[e], x[e].w, sum.w);
     }
   }
-  if (split > 1) {  // no CTA leaves while another still reads its partials
-    __syncwarp();
-    cluster_sync_all();
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) l += __shfl_xor_sync(0xffffffffu, l, offset);
+  if constexpr (kRowWarps > 1) {
+    __shared__ float4 other_sum[kRowWarps][kDim / 4];
+    __shared__ float2 other_ml[kRowWarps];
+    if (active) other_sum[part][lane] = sum;
+    if (lane == 0) other_ml[part] = make_float2(m, l);
+    __syncthreads();
+    if (part != 0) return;
+    float highest = m;
+#pragma unroll
+    for (int w = 1; w < kRowWarps; ++w) highest = fmaxf(highest, other_ml[w].x);
+    l = 0.f, sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const float weight = other_ml[w].x == -INFINITY ? 0.f : exp2_approx(other_ml[w].x - highest);
+      if (weight == 0.f) continue;
+      l += weight * other_ml[w].y;
+      if (active) {
+        const float4 x = other_sum[w][lane];
+        sum.x = fmaf(weight, x.x, sum.x), sum.y = fmaf(weight, x.y, sum.y), sum.z = fmaf(weight, x.z, sum.z), sum.w = fmaf(weight, x.w, sum.w);
+      }
+    }
+  }
+  const float reciprocal = l == 0.f ? 0.f : 1.f / l;  // no key: zeros
+  if (there && active && lane * 4 < a.head_dim) {
+    T* out = static_cast<T*>(a.out) + t * a.o_st + head * a.o_sh + lane * 4;
+    *reinterpret_cast<uint2*>(out) = make_uint2(prefix_pack<T>(sum.x * reciprocal, sum.y * reciprocal), prefix_pack<T>(sum.z * reciprocal, sum.w * reciprocal));
   }
 }
 
