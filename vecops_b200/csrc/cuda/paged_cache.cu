@@ -98,7 +98,7 @@ struct PrefixPlan {
   bool fast = false;  // the two kernels can address this call; the one-warp-per-row kernel serves the rest
   int dim = 0;        // head dims a kernel is built for: 64 or 128
   int both_rows = 0, row_blocks = 0, tiles = 0, tiles_per_chunk = 0, chunks = 0, records = 0;
-  int tokens_per_item = 1, group_tiles = 1, slot_shift = 0, workers = 0;
+  int tokens_per_item = 1, group_tiles = 1, workers = 0;
   int64_t slots = 0, fragments = 0;
   uint64_t ml_at = 0, fragment_o_at = 0, fragment_ml_at = 0, sums_at = 0, total = 0;
 };
@@ -138,9 +138,12 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
   p.tokens_per_item = static_cast<int>(group <= 16 ? 16 / group : 1);
   p.group_tiles = static_cast<int>((group + 15) / 16);
   p.slots = a.query_starts == nullptr ? a.batch : a.tokens / p.tokens_per_item + a.batch + 1;
-  while ((p.slots >> p.slot_shift) >= SuffixSdpa<64>::kTableSlots) ++p.slot_shift;
-  // warps for every slice the table could hold, up to what the SMs hold at once
+  // warps for every slice the table could hold, up to what the SMs hold at once (slices are counted in 32 bits)
   const int64_t slices = (a.table_width * a.page_size + 15) / 16, columns = a.kv_heads * p.group_tiles;
+  if (slices > 0 && p.slots * columns > ((INT64_C(1) << 31) - 1) / (slices + kItemWeight)) {
+    p.fast = false;
+    return p;
+  }
   const int64_t most = static_cast<int64_t>(sms) * SuffixSdpa<64>::kCtasPerSm * SuffixSdpa<64>::kWarps;
   int64_t wanted = p.slots * columns;
   wanted = slices == 0 || wanted >= most ? (slices == 0 ? 1 : most) : (wanted * slices < most ? wanted * slices : most);
@@ -175,7 +178,8 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   static std::atomic<bool> raised[64];
   if (device.index >= 64 || !raised[device.index].load()) {
     cudaError_t status = cudaFuncSetAttribute(prefix_sdpa_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmemBytes);
-    if (status == cudaSuccess) status = cudaFuncSetAttribute(suffix_sdpa_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, SuffixSdpa<kDim>::kSmemBytes);
+    if (status == cudaSuccess) status = cudaFuncSetAttribute(suffix_sdpa_kernel<T, kDim, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SuffixSdpa<kDim>::kSmemBytes);
+    if (status == cudaSuccess) status = cudaFuncSetAttribute(suffix_sdpa_kernel<T, kDim, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SuffixSdpa<kDim>::kSmemBytes);
     if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "cudaFuncSetAttribute(prefix_sdpa): %s", cudaGetErrorString(status));
     if (device.index < 64) raised[device.index].store(true);
   }
@@ -215,7 +219,7 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   s.a = args;
   s.rows = rows;
   s.tokens_per_item = plan.tokens_per_item, s.group_tiles = plan.group_tiles;
-  s.slots = static_cast<int>(plan.slots), s.slot_shift = plan.slot_shift, s.workers = plan.workers;
+  s.slots = static_cast<int>(plan.slots), s.workers = plan.workers;
   s.records = plan.records, s.partial_o = partial_o, s.partial_ml = partial_ml;
   char* base = static_cast<char*>(a.workspace);
   s.fragment_o = reinterpret_cast<float*>(base + plan.fragment_o_at), s.fragment_ml = reinterpret_cast<float2*>(base + plan.fragment_ml_at);
@@ -224,13 +228,13 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   config.blockDim = dim3(SuffixSdpa<kDim>::kThreads);
   config.dynamicSmemBytes = SuffixSdpa<kDim>::kSmemBytes;
   config.numAttrs = 1;
-  cudaError_t status = cudaLaunchKernelEx(&config, suffix_sdpa_kernel<T, kDim>, s);
+  cudaError_t status = a.page_size % 16 == 0 ? cudaLaunchKernelEx(&config, suffix_sdpa_kernel<T, kDim, true>, s) : cudaLaunchKernelEx(&config, suffix_sdpa_kernel<T, kDim, false>, s);
   if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "suffix_sdpa launch: %s", cudaGetErrorString(status));
   int32_t rc = decode_launched("suffix_sdpa", error);
   if (rc != VECOPS_STATUS_OK) return rc;
   // few rows: four warps share one's partial results
   const int64_t out_rows = a.tokens * a.q_heads;
-  const bool shared_rows = out_rows <= static_cast<int64_t>(device.sms) * 16;
+  const bool shared_rows = out_rows <= static_cast<int64_t>(device.sms) * 4;
   const int64_t blocks = shared_rows ? out_rows : (out_rows + 3) / 4;
   if (blocks > 0x7fffffff) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
   config.gridDim = dim3(static_cast<unsigned>(blocks));

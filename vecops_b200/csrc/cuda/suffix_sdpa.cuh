@@ -4,7 +4,7 @@
 // An item is up to sixteen query rows of one sequence and one key/value head - the queries that read this head, of one
 // token or of a few neighbouring ones - and the keys they see, in slices of sixteen.  The work is the keys' way from
 // memory: every key and value is used by at most sixteen rows.  So all slices of all items, in order, are dealt out evenly to
-// the warps of the grid whatever the lengths are; a warp keeps the next slice in flight by cp.async while it multiplies
+// the warps of the grid whatever the lengths are - an item counts as kItemWeight slices more, for what starting on it costs; a warp keeps the next slice in flight by cp.async while it multiplies
 // one with mma.sync m16n8k16, whose sixteen rows are the item's (tcgen05's 128 would be nearly empty).  Warps share
 // nothing and meet at no barrier.  Each runs m' = max(m, s), l, O over its part of an item and leaves them as a fragment;
 // sdpa_merge_rows_kernel, launched behind, joins a row's fragments and its prefix records,
@@ -29,9 +29,7 @@ struct SuffixSdpa {
   static constexpr int kWarpBytes = kStages * 2 * kTileBytes;
   static constexpr int kProbOffset = kWarps * kWarpBytes;
   static constexpr int kProbBytes = kRows * kKeys * 4;  // per warp: probabilities of the keys that only some rows see
-  static constexpr int kTableOffset = kProbOffset + kWarps * kProbBytes;
-  static constexpr int kTableSlots = 1024;              // running sums of the items' slices; more items share an entry
-  static constexpr int kSmemBytes = kTableOffset + (kTableSlots + 1 + kWarps * kStages + 32) * 4;
+  static constexpr int kSmemBytes = kProbOffset + kWarps * kProbBytes + kWarps * kStages * 4;
 };
 
 struct SuffixSdpaArgs {
@@ -40,22 +38,18 @@ struct SuffixSdpaArgs {
   int tokens_per_item;  // neighbouring tokens of one sequence in an item
   int group_tiles;      // items a token is cut into when its group has more than sixteen heads
   int slots;            // of items per (head, group tile), idle ones included
-  int slot_shift;       // log2 of the slots that share an entry of the table
   int workers;          // warps of the suffix kernel
   int records;          // of the prefix kernel
   const float* partial_o;
   const float2* partial_ml;
   float* fragment_o;    // [warp + item][16][kDim]
   float2* fragment_ml;  // [warp + item][16]
-  int* sums;            // [slot] slices of the slots before it, written where the slot has any; then [slots] the sum of all
+  int* sums;            // [slot] weight of the slots before it, written where the slot has any; then [slots] the sum of all
 };
 
-// What a slot holds.  Without query_starts slot b is sequence b's one token; with them sequence b's items are the slots from
+// Without query_starts slot b is sequence b's one token; with them sequence b's items are the slots from
 // query_starts[b] / tokens_per_item + b on: apart from each other, and found without a sum.
-struct SuffixItem {
-  int sequence, first, count;  // tokens [first, first + count); count 0: an idle slot
-  int newest, length;
-};
+constexpr int kItemWeight = 2;  // slices' worth of time that an item's lookups, queries and fragment take (measured: 2.5 us of 1 to 2 us each)
 
 __device__ __forceinline__ int suffix_sees(const PrefixSdpaArgs& a, int length, int newest, int t) {
   const long long capacity = static_cast<long long>(a.table_width) * a.page_size;
@@ -77,18 +71,11 @@ __device__ __forceinline__ int suffix_search(int batch, const Before& before) {
   return low;
 }
 
-__device__ __forceinline__ SuffixItem suffix_item(const SuffixSdpaArgs& p, int slot) {
-  SuffixItem item{slot, slot, 1, slot, -1};
-  if (p.a.query_starts != nullptr) {
-    item.sequence = suffix_search(p.a.batch, [&](int b) { return p.a.query_starts[b] / p.tokens_per_item + b <= slot; });
-    const int start = p.a.query_starts[item.sequence], end = p.a.query_starts[item.sequence + 1];
-    item.first = start + (slot - (start / p.tokens_per_item + item.sequence)) * p.tokens_per_item;
-    item.count = min(p.tokens_per_item, end - item.first);
-    item.newest = end - 1;
-  }
-  item.length = p.a.lengths[item.sequence];
-  return item;
+// Slices and weight of the item whose newest token is `last`.
+__device__ __forceinline__ int suffix_slices(const PrefixSdpaArgs& a, int length, int newest, int last) {
+  return length <= 0 ? 0 : (suffix_sees(a, length, newest, last) + 15) / 16;
 }
+__device__ __forceinline__ int suffix_weight(int slices) { return slices > 0 ? slices + kItemWeight : 0; }
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -131,159 +118,158 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) {
   return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
-template <typename T, int kDim>
+// kWholePages: page_size is a multiple of sixteen, so a slice lies in one page.
+template <typename T, int kDim, bool kWholePages>
 __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::kCtasPerSm) suffix_sdpa_kernel(const SuffixSdpaArgs p) {
   using G = SuffixSdpa<kDim>;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t smem_base = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PrefixSdpaArgs& a = p.a;
-  int* table = reinterpret_cast<int*>(smem + G::kTableOffset);  // [entry] slices of the slots before the entry's
-  volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(table + G::kTableSlots + 1) + warp * G::kStages;
-  int* warp_sums = table + G::kTableSlots + 1 + G::kWarps * G::kStages;
+  volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(smem + G::kProbOffset + G::kWarps * G::kProbBytes) + warp * G::kStages;
   if (p.records == 0) grid_dependency_wait();  // (with a prefix kernel in between, the kernels before that one are done already)
   grid_launch_dependents();
 
-  // ---------------------------------------------------------------- how many slices come before each slot
-  const int entries = (p.slots + (1 << p.slot_shift) - 1) >> p.slot_shift;
-  for (int e = threadIdx.x; e < G::kTableSlots + 1; e += G::kThreads) table[e] = 0;
-  __syncthreads();
-  for (int b = threadIdx.x; b < a.batch; b += G::kThreads) {
+  // ---------------------------------------------------------------- this warp's positions [position, end)
+  // Every warp adds the weights up for itself, a lane per run of sequences: no barrier, one trip to memory for a small batch.
+  struct Tokens {
+    int begin, end;  // of a sequence
+  };
+  auto tokens_of = [&](int b) -> Tokens {
+    if (a.query_starts == nullptr) return {b, b + 1};
+    return {max(0, a.query_starts[b]), min(a.tokens, a.query_starts[b + 1])};
+  };
+  const int per_lane = (a.batch + 31) / 32;
+  int sum = 0;
+  for (int b = lane * per_lane; b < min(a.batch, (lane + 1) * per_lane); ++b) {
     const int length = a.lengths[b];
-    if (length <= 0) continue;
-    if (a.query_starts == nullptr) {
-      atomicAdd(table + (b >> p.slot_shift), (suffix_sees(a, length, b, b) + G::kKeys - 1) / G::kKeys);
-    } else {
-      const int start = max(0, a.query_starts[b]), end = min(a.tokens, a.query_starts[b + 1]);
-      int slot = start / p.tokens_per_item + b;
-      for (int first = start; first < end && slot < p.slots; first += p.tokens_per_item, ++slot)
-        atomicAdd(table + (slot >> p.slot_shift), (suffix_sees(a, length, end - 1, min(end, first + p.tokens_per_item) - 1) + G::kKeys - 1) / G::kKeys);
-    }
+    const Tokens tokens = tokens_of(b);
+    for (int first = tokens.begin; first < tokens.end; first += p.tokens_per_item)
+      sum += suffix_weight(suffix_slices(a, length, tokens.end - 1, min(tokens.end, first + p.tokens_per_item) - 1));
   }
-  __syncthreads();
-  {
-    // exclusive sums over the entries, eight a thread
-    constexpr int kMine = G::kTableSlots / G::kThreads;
-    int mine[kMine], sum = 0;
+  int before = sum;
 #pragma unroll
-    for (int e = 0; e < kMine; ++e) mine[e] = table[threadIdx.x * kMine + e], sum += mine[e];
-    int before = sum;
-#pragma unroll
-    for (int offset = 1; offset < 32; offset <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, before, offset);
-      if (lane >= offset) before += other;
-    }
-    if (lane == 31) warp_sums[warp] = before;
-    __syncthreads();
-    before -= sum;
-    for (int w = 0; w < warp; ++w) before += warp_sums[w];
-#pragma unroll
-    for (int e = 0; e < kMine; ++e) table[threadIdx.x * kMine + e] = before, before += mine[e];
-    if (threadIdx.x == G::kThreads - 1) table[G::kTableSlots] = before;
-    __syncthreads();
+  for (int offset = 1; offset < 32; offset <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, before, offset);
+    if (lane >= offset) before += other;
   }
+  const int total = __shfl_sync(0xffffffffu, before, 31);
+  before -= sum;
   const int columns = a.kv_heads * p.group_tiles;  // items of a slot
-  const long long all = static_cast<long long>(table[G::kTableSlots]) * columns;
+  const int all = total * columns;                 // (the host has made sure that it fits)
   const int worker = static_cast<int>(blockIdx.x) * G::kWarps + warp;
-  if (worker == 0 && lane == 0) p.sums[p.slots] = table[G::kTableSlots];
-
-  // ---------------------------------------------------------------- this warp's slices [position, end)
-  const long long workers = min(static_cast<long long>(p.workers), all);  // (no warp is dealt nothing while another has something)
-  long long position = worker < workers ? all * worker / workers : 0;
-  const long long end = worker < workers ? all * (worker + 1) / workers : 0;
+  if (worker == 0 && lane == 0) p.sums[p.slots] = total;
+  const int workers = min(p.workers, all);  // (no warp is dealt nothing while another has something)
+  int position = worker < workers ? static_cast<int>(static_cast<long long>(all) * worker / workers) : 0;
+  const int end = worker < workers ? static_cast<int>(static_cast<long long>(all) * (worker + 1) / workers) : 0;
+  // the run of sequences that the first position lies in, to be walked from its first
+  const int in_run = 31 - __clz(__ballot_sync(0xffffffffu, before <= position / columns) | 1u);
+  int slot_sum = __shfl_sync(0xffffffffu, before, in_run);  // weight of the slots before `slot`
+  int sequence = in_run * per_lane, length = 0, slices = 0, weight = 0, slot = 0, first = 0;
+  Tokens tokens{0, 0};
+  if (position < end) {
+    tokens = tokens_of(sequence), length = a.lengths[sequence];
+    first = tokens.begin, slot = a.query_starts != nullptr ? first / p.tokens_per_item + sequence : sequence;
+  }
   const uint32_t ring = smem_base + warp * G::kWarpBytes;
   float* probabilities = reinterpret_cast<float*>(smem + G::kProbOffset + warp * G::kProbBytes);
   while (position < end) {
-    // the slot: by the table, and where several share an entry by counting on from its first
-    const int before_slot = static_cast<int>(position / columns);  // (a slot's items have the same number of slices)
-    int low = 0, high = entries;
-    while (high - low > 1) {
-      const int middle = (low + high) / 2;
-      if (table[middle] <= before_slot) low = middle;
-      else high = middle;
+    for (;;) {  // on to the slot that has the position
+      if (first < tokens.end) {
+        slices = suffix_slices(a, length, tokens.end - 1, min(tokens.end, first + p.tokens_per_item) - 1);
+        weight = suffix_weight(slices);
+        if (position < (slot_sum + weight) * columns) break;
+        slot_sum += weight;
+        first += p.tokens_per_item, ++slot;
+      } else {
+        if (++sequence >= a.batch) break;  // (the sums agree with the walk: not reached)
+        tokens = tokens_of(sequence), length = a.lengths[sequence];
+        first = tokens.begin, slot = a.query_starts != nullptr ? first / p.tokens_per_item + sequence : sequence;
+      }
     }
-    int slot = low << p.slot_shift, slot_sum = table[low], slices = 0;
-    SuffixItem item;
-    for (;; ++slot) {
-      item = suffix_item(p, slot);
-      const bool idle = item.count <= 0 || item.first < 0 || item.first + item.count > a.tokens || item.length <= 0 ||
-                        (a.query_starts != nullptr && item.first < a.query_starts[item.sequence]);
-      slices = idle ? 0 : (suffix_sees(a, item.length, item.newest, item.first + item.count - 1) + G::kKeys - 1) / G::kKeys;
-      if (before_slot < slot_sum + slices || slot + 1 >= p.slots) break;
-      slot_sum += slices;
-    }
-    if (slices <= 0) break;  // (the table and this count agree: not reached)
+    if (sequence >= a.batch) break;
     if (lane == 0) p.sums[slot] = slot_sum;
-    const long long in_slot = position - static_cast<long long>(slot_sum) * columns;
-    const int column = static_cast<int>(in_slot / slices), first_slice = static_cast<int>(in_slot - static_cast<long long>(column) * slices);
-    const int mine = static_cast<int>(min(static_cast<long long>(slices - first_slice), end - position));
-    position += mine;
+    const int in_slot = position - slot_sum * columns;
+    const int column = in_slot / weight, in_item = in_slot - column * weight;
+    const int stop = min(weight, in_item + end - position);
+    position += stop - in_item;
+    const int first_slice = max(0, in_item - kItemWeight), mine = max(0, stop - kItemWeight) - first_slice;
+    if (mine <= 0) continue;  // (only the item's extra weight was dealt to this warp)
+    const int count = min(p.tokens_per_item, tokens.end - first);
     const int kv = column / p.group_tiles, group0 = column % p.group_tiles * 16;
-    const int heads = min(16, a.group - group0), rows = item.count * heads;  // rows are [token][head in group]
-    const int first = item.first;
-    auto sees_of = [&](int t) { return suffix_sees(a, item.length, item.newest, t); };
-    const int all_see = sees_of(first), some_see = sees_of(first + item.count - 1);
+    const int heads = min(16, a.group - group0), rows = count * heads;  // rows are [token][head in group]
+    auto sees_of = [&](int t) { return suffix_sees(a, length, tokens.end - 1, t); };
+    const int all_see = sees_of(first), some_see = sees_of(first + count - 1);
 
     const T* k_base = static_cast<const T*>(a.k) + kv * a.k_sh;
     const T* v_base = static_cast<const T*>(a.v) + kv * a.v_sh;
-    const int* pages = a.page_table + item.sequence * a.table_stride;
-    auto page_of = [&](int i) {  // page of this lane's key (lanes 0..15) in slice i, or -1
-      const int key = (first_slice + i) * G::kKeys + (lane & 15);
-      return i < mine && key < some_see ? __ldg(pages + key / a.page_size) : -1;
-    };
+    const int* pages = a.page_table + sequence * a.table_stride;
     constexpr int kPieces = kDim / 8;           // 16-byte pieces of a row
     constexpr int kRowsPerStep = 32 / kPieces;  // rows a warp-wide copy covers
-    int page_next = page_of(0), page_after = page_of(1);
+    const int piece = lane % kPieces, sub_row = lane / kPieces;
+    // pages of the next two slices, looked up ahead: the slice's own, or - pages that end inside a slice - that of this lane's key (lanes 0..15)
+    int page_slot = 0, page_offset = 0;  // where the slice to be looked up next starts
+    if constexpr (kWholePages) page_slot = first_slice * G::kKeys / a.page_size, page_offset = first_slice * G::kKeys - page_slot * a.page_size;
+    int look = 0;
+    auto page_of_next = [&] {
+      int page = -1;
+      if constexpr (kWholePages) {
+        if (look < mine && page_slot < a.table_width) page = __ldg(pages + page_slot);
+        page_offset += G::kKeys;
+        if (page_offset >= a.page_size) page_offset = 0, ++page_slot;
+      } else {
+        const int key = (first_slice + look) * G::kKeys + (lane & 15);
+        if (look < mine && key < some_see) page = __ldg(pages + key / a.page_size);
+      }
+      ++look;
+      return page;
+    };
+    int offset_next = page_offset;
+    int page_next = page_of_next(), page_after = page_of_next();
     auto issue = [&](int i) {
-      const int stage = i % G::kStages;
-      const int page = page_next;
-      page_next = page_after;
-      page_after = page_of(i + 2);
       if (i < mine) {
-        const int key = (first_slice + i) * G::kKeys + (lane & 15);
+        const int stage = i % G::kStages, page = page_next;
+        page_next = page_after;
+        page_after = page_of_next();
         const bool there = page >= 0 && page < a.pages;
-        const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
+        const uint32_t dst = ring + stage * 2 * G::kTileBytes + sub_row * G::kRowBytes;
+        uint32_t mask;
+        long long k_at = 0, v_at = 0;
+        if constexpr (kWholePages) {
+          const int keys = min(G::kKeys, some_see - (first_slice + i) * G::kKeys);
+          mask = there ? 0xffffu >> (16 - keys) : 0u;
+          if (there) {
+            k_at = page * a.k_sp + (offset_next + sub_row) * a.k_ss, v_at = page * a.v_sp + (offset_next + sub_row) * a.v_ss;
+          }
+          offset_next += G::kKeys;
+          if (offset_next >= a.page_size) offset_next = 0;
+        } else {
+          mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
+          const long long offset = ((first_slice + i) * G::kKeys + (lane & 15)) % a.page_size;
+          if (there) k_at = page * a.k_sp + offset * a.k_ss, v_at = page * a.v_sp + offset * a.v_ss;
+        }
         if (lane == 0) present[stage] = mask;
-        const long long offset = key % a.page_size;
-        const long long k_at = there ? page * a.k_sp + offset * a.k_ss : 0, v_at = there ? page * a.v_sp + offset * a.v_ss : 0;
-        const uint32_t dst = ring + stage * 2 * G::kTileBytes;
-        const int piece = lane % kPieces;
+        const T *k_from = k_base + k_at, *v_from = v_base + v_at;
 #pragma unroll
         for (int step = 0; step < G::kKeys / kRowsPerStep; ++step) {
-          const int row = step * kRowsPerStep + lane / kPieces;
-          const long long k_row = __shfl_sync(0xffffffffu, k_at, row), v_row = __shfl_sync(0xffffffffu, v_at, row);
+          const int row = step * kRowsPerStep + sub_row;
+          if constexpr (!kWholePages) {
+            k_from = k_base + __shfl_sync(0xffffffffu, k_at, row);
+            v_from = v_base + __shfl_sync(0xffffffffu, v_at, row);
+          }
+          // (nothing is read where the size is 0: the address may be any)
           const uint32_t bytes = (mask >> row & 1u) != 0 && piece * 8 < a.head_dim ? 16 : 0;
-          const uint32_t to = dst + row * G::kRowBytes + ((piece ^ (row & 7)) << 4);
-          cp_async_16(to, k_base + k_row + (bytes != 0 ? piece * 8 : 0), bytes);
-          cp_async_16(to + G::kTileBytes, v_base + v_row + (bytes != 0 ? piece * 8 : 0), bytes);
+          const uint32_t to = dst + step * kRowsPerStep * G::kRowBytes + ((piece ^ (row & 7)) << 4);
+          cp_async_16(to, bytes != 0 ? k_from + piece * 8 : k_base, bytes);
+          cp_async_16(to + G::kTileBytes, bytes != 0 ? v_from + piece * 8 : v_base, bytes);
+          if constexpr (kWholePages) k_from += kRowsPerStep * a.k_ss, v_from += kRowsPerStep * a.v_ss;
         }
       }
       cp_async_commit();
     };
-#pragma unroll
-    for (int i = 0; i < G::kStages - 1; ++i) issue(i);
 
-    // Q: the A fragments of sixteen rows
     const int r_low = lane >> 2, r_high = r_low + 8;
     uint32_t q[kDim / 16][4];
-    {
-      const T* q_row[2];
-      bool there[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = h == 0 ? r_low : r_high;
-        there[h] = r < rows;
-        const int t = first + (there[h] ? r / heads : 0), head = kv * a.group + group0 + (there[h] ? r % heads : 0);
-        q_row[h] = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
-      }
-#pragma unroll
-      for (int ks = 0; ks < kDim / 16; ++ks)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = ks * 16 + (lane & 3) * 2 + (e >> 1) * 8;
-          q[ks][e] = there[e & 1] && d < a.head_dim ? *reinterpret_cast<const uint32_t*>(q_row[e & 1] + d) : 0u;
-        }
-    }
     const int sees[2] = {r_low < rows ? sees_of(first + r_low / heads) : 0, r_high < rows ? sees_of(first + r_high / heads) : 0};
     const float scale = a.scale * 1.4426950408889634f;
     float o[kDim / 8][4];
@@ -293,8 +279,30 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
       for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    for (int i = 0; i < mine; ++i) {
+    for (int i = 1 - G::kStages; i < mine; ++i) {
       issue(i + G::kStages - 1);
+      if (i < 0) {
+        // Q, behind the first copies: the A fragments of sixteen rows
+        {
+          const T* q_row[2];
+          bool there[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = h == 0 ? r_low : r_high;
+            there[h] = r < rows;
+            const int t = first + (there[h] ? r / heads : 0), head = kv * a.group + group0 + (there[h] ? r % heads : 0);
+            q_row[h] = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
+          }
+#pragma unroll
+          for (int ks = 0; ks < kDim / 16; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d = ks * 16 + (lane & 3) * 2 + (e >> 1) * 8;
+              q[ks][e] = there[e & 1] && d < a.head_dim ? *reinterpret_cast<const uint32_t*>(q_row[e & 1] + d) : 0u;
+            }
+        }
+        continue;
+      }
       cp_async_wait<G::kStages - 1>();
       __syncwarp();
       const int stage = i % G::kStages, key0 = (first_slice + i) * G::kKeys;
@@ -441,60 +449,56 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
     const int tile = (t - start) / p.tokens_per_item, first = start + tile * p.tokens_per_item;
     const int slot = a.query_starts != nullptr ? start / p.tokens_per_item + sequence + tile : sequence;
     const int last = min(newest, first + p.tokens_per_item - 1);
-    const int slices = (suffix_sees(a, length, newest, last) + 15) / 16;
+    const int slices = suffix_slices(a, length, newest, last), weight = suffix_weight(slices);
     if (slices > 0) {
       const int columns = a.kv_heads * p.group_tiles, column = kv * p.group_tiles + in_group / 16;
-      const long long all = static_cast<long long>(__ldcg(p.sums + p.slots)) * columns;
-      const long long from = static_cast<long long>(__ldcg(p.sums + slot)) * columns + static_cast<long long>(column) * slices;
-      const long long workers = min(static_cast<long long>(p.workers), all);
-      auto worker_of = [&](long long slice) { return ((slice + 1) * workers - 1) / all; };  // whose [all w / workers, all (w + 1) / workers) has it
-      const long long first_worker = worker_of(from);
-      fragments = static_cast<int>(worker_of(from + slices - 1) - first_worker) + 1;
+      const int all = __ldcg(p.sums + p.slots) * columns, from = __ldcg(p.sums + slot) * columns + column * weight, workers = min(p.workers, all);
+      auto worker_of = [&](int at) { return static_cast<int>(((at + 1ll) * workers - 1) / all); };  // whose [all w / workers, all (w + 1) / workers) has it
+      const int first_worker = worker_of(from + kItemWeight);  // (the item's extra weight lies before its slices)
+      fragments = worker_of(from + weight - 1) - first_worker + 1;
       const int heads = min(16, a.group - in_group / 16 * 16);
       first_fragment = (static_cast<size_t>(first_worker) + static_cast<size_t>(slot) * columns + column) * 16 + (t - first) * heads + in_group % 16;
     }
   }
-  const size_t record_row = static_cast<size_t>(kv) * p.rows + static_cast<size_t>(t) * a.group + in_group;
-  const size_t record_step = static_cast<size_t>(a.kv_heads) * p.rows;
-  const int sources = owned ? fragments + p.records : 0;
-  auto ml_of = [&](int c) {
-    return c < fragments ? __ldcg(p.fragment_ml + first_fragment + static_cast<size_t>(c) * 16) : __ldcg(p.partial_ml + (c - fragments) * record_step + record_row);
-  };
-  auto o_of = [&](int c) {
-    return c < fragments ? p.fragment_o + (first_fragment + static_cast<size_t>(c) * 16) * kDim : p.partial_o + ((c - fragments) * record_step + record_row) * kDim;
-  };
-
-  // ---- this warp's share: a block of sources at a time, a lane per (m, l), four dims a lane
-  constexpr int kBlock = kRowWarps > 1 ? 8 : 32;
+  // ---- this warp's share: eight partial results at a time, a lane per (m, l), four dims a lane, all their loads together
   const bool active = lane * 4 < kDim;
   float m = -INFINITY, l = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c0 = part * kBlock; c0 < sources; c0 += kRowWarps * kBlock) {
-    const int here = min(kBlock, sources - c0);
-    const float2 ml = lane < here ? ml_of(c0 + lane) : make_float2(-INFINITY, 0.f);
-    float highest = ml.x;
-#pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, offset));
-    if (highest == -INFINITY) continue;
-    const float m_new = fmaxf(m, highest), keep = m == -INFINITY ? 0.f : exp2_approx(m - m_new);
-    m = m_new;
-    const float weight = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - m);
-    l = l * keep + weight * ml.y;
-    sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
-    for (int c = 0; c < here; c += 8) {
+  auto join = [&](int count, const float2* ml_at, const float* o_at, size_t step) {  // partial c: ml_at[c * step], o_at[c * step * kDim]
+#pragma unroll 1
+    for (int c0 = part * 8; c0 < count; c0 += kRowWarps * 8) {
+      const int here = min(8, count - c0);
+      const float2 ml = lane < here ? __ldcg(ml_at + (c0 + lane) * step) : make_float2(-INFINITY, 0.f);
       float4 x[8];
-      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = e < here && active ? __ldcg(reinterpret_cast<const float4*>(o_at + (c0 + e) * step * kDim) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float highest = ml.x;
+#pragma unroll
+      for (int offset = 4; offset > 0; offset >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, offset));
+      highest = __shfl_sync(0xffffffffu, highest, 0);
+      if (highest == -INFINITY) continue;  // (the same for the warp)
+      const float m_new = fmaxf(m, highest), keep = m == -INFINITY ? 0.f : exp2_approx(m - m_new);
+      m = m_new;
+      const float weight = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - m);
+      l = l * keep + weight * ml.y;
+      sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        w[e] = __shfl_sync(0xffffffffu, weight, (c + e) & 31);  // (0 past the last)
-        x[e] = w[e] != 0.f && active ? __ldcg(reinterpret_cast<const float4*>(o_of(c0 + c + e)) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float w = __shfl_sync(0xffffffffu, weight, e);
+        if (w != 0.f)  // (a partial result without a key may hold anything)
+          sum.x = fmaf(w, x[e].x, sum.x), sum.y = fmaf(w, x[e].y, sum.y), sum.z = fmaf(w, x[e].z, sum.z), sum.w = fmaf(w, x[e].w, sum.w);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum.x = fmaf(w[e], x[e].x, sum.x), sum.y = fmaf(w[e], x[e].y, sum.y), sum.z = fmaf(w[e], x[e].z, sum.z), sum.w = fmaf(w[e], x[e].w, sum.w);
     }
+  };
+  const size_t record_row = static_cast<size_t>(kv) * p.rows + static_cast<size_t>(t) * a.group + in_group;
+  if (owned) {
+    join(p.records, p.partial_ml + record_row, p.partial_o + record_row * kDim, static_cast<size_t>(a.kv_heads) * p.rows);
+    join(fragments, p.fragment_ml + first_fragment, p.fragment_o + first_fragment * kDim, 16);
   }
 #pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) l += __shfl_xor_sync(0xffffffffu, l, offset);
+  for (int offset = 4; offset > 0; offset >>= 1) l += __shfl_xor_sync(0xffffffffu, l, offset);  // (the first eight lanes')
+  l = __shfl_sync(0xffffffffu, l, 0);
   if constexpr (kRowWarps > 1) {
     __shared__ float4 other_sum[kRowWarps][kDim / 4];
     __shared__ float2 other_ml[kRowWarps];
