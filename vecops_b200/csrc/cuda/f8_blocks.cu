@@ -27,10 +27,11 @@ int32_t quantize_typed(const VecopsB200QuantizeBlocks& q, int sms, VecopsError* 
   cudaStream_t stream = static_cast<cudaStream_t>(q.stream);
   const int64_t col_blocks = (q.cols + 127) / 128;
   if (q.block_rows == 1) {
-    const int64_t want = (q.rows * col_blocks + 15) / 16;
-    const unsigned grid = static_cast<unsigned>(want < static_cast<int64_t>(sms) * 64 ? want : static_cast<int64_t>(sms) * 64);
-    if (vec) f8_quantize_rows_kernel<T, true><<<grid, 256, 0, stream>>>(p);
-    else f8_quantize_rows_kernel<T, false><<<grid, 256, 0, stream>>>(p);
+    const int64_t blocks = q.rows * col_blocks, per_cta = vec ? 32 : 16, most = static_cast<int64_t>(sms) * 8;
+    const int64_t want = (blocks + per_cta - 1) / per_cta;
+    const unsigned grid = static_cast<unsigned>(want < most ? want : most);
+    if (vec) f8_quantize_rows_kernel<T><<<grid, 256, 0, stream>>>(p);
+    else f8_quantize_strided_kernel<T><<<grid, 256, 0, stream>>>(p);
     return decode_launched("quantize_blocks", error);
   }
   const dim3 grid(static_cast<unsigned>(col_blocks), static_cast<unsigned>((q.rows + 127) / 128));

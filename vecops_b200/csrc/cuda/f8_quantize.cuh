@@ -12,6 +12,8 @@
 #include <float.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace vb200 {
 
 struct F8Quantize {
@@ -79,9 +81,118 @@ struct F8QuantizeArgs {
   long long rows, cols;
 };
 
-// 1 x 128 blocks: sixteen threads per block, eight elements each.
+// The largest of amax and eight elements that still lie as they were loaded; a NaN does not count.
+template <typename T>
+__device__ __forceinline__ float f8_raw_amax(const uint4& raw) {
+  if constexpr (sizeof(T) == 2) {
+    // two at a time: the sign bits off, packed maxima
+    uint32_t top = raw.x & 0x7fff7fffu;
+    const uint32_t words[3] = {raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint32_t w = words[i] & 0x7fff7fffu;
+      if constexpr (std::is_same<T, __half>::value) asm("max.f16x2 %0, %0, %1;" : "+r"(top) : "r"(w));
+      else asm("max.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(w));
+    }
+    const T* pair = reinterpret_cast<const T*>(&top);
+    return fmaxf(f8_source(pair[0]), f8_source(pair[1]));
+  } else {
+    const float* x = reinterpret_cast<const float*>(&raw);
+    return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+  }
+}
+
+// The 16 bytes' worth of elements, scaled, rounded and stored; `left` of them are inside the row.
 template <typename T, bool kVec>
+__device__ __forceinline__ void f8_store_raw(uint8_t* dst, const uint4& raw, float factor, int left) {
+  constexpr int kPerLoad = 16 / sizeof(T);
+  const T* x = reinterpret_cast<const T*>(&raw);
+  uint32_t words[kPerLoad / 4];
+#pragma unroll
+  for (int w = 0; w < kPerLoad / 4; ++w) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f8_source(x[4 * w]) * factor, f8_source(x[4 * w + 1]) * factor), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f8_source(x[4 * w + 2]) * factor, f8_source(x[4 * w + 3]) * factor), __NV_SATFINITE, __NV_E4M3);
+    words[w] = lo | hi << 16;
+  }
+  if (kVec && left >= kPerLoad) {
+    if constexpr (kPerLoad == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(words[0], words[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = words[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPerLoad; ++e)
+      if (e < left) dst[e] = static_cast<uint8_t>(words[e >> 2] >> (8 * (e & 3)));
+  }
+}
+
+// 1 x 128 blocks of rows that allow 16-byte loads: eight threads a block, the elements held as loaded between the maximum
+// and the conversion; two blocks' loads in flight per thread.  One division a block gives both the factor (lanes 0..6) and the
+// scale (lane 7).  Instructions bound it as much as memory does: 20 an element, in a first form that converted before it
+// compared and divided twice, moved 3.0 TB/s.
+template <typename T>
 __global__ void __launch_bounds__(256) f8_quantize_rows_kernel(const F8QuantizeArgs p) {
+  constexpr int kPerLoad = 16 / sizeof(T), kLoads = F8Quantize::kBlock / 8 / kPerLoad, kTogether = sizeof(T) == 4 ? 1 : 2;
+  const int col_blocks = static_cast<int>((p.cols + F8Quantize::kBlock - 1) / F8Quantize::kBlock);
+  const int lane = threadIdx.x & 7;
+  const unsigned members = 0xffu << (threadIdx.x & 24);
+  // blocks are counted along the rows; from one to this thread group's next one by adding, not by dividing
+  const long long step = gridDim.x * 32ll;
+  const long long step_rows = step / col_blocks;
+  const int step_cols = static_cast<int>(step - step_rows * col_blocks);
+  const long long start = blockIdx.x * 32ll + (threadIdx.x >> 3);
+  long long row = start / col_blocks;
+  int col_block = static_cast<int>(start - row * col_blocks);
+  while (row < p.rows) {
+    uint4 raw[kTogether][kLoads];
+    long long rows[kTogether];
+    int cols[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      rows[i] = row, cols[i] = col_block;
+      const T* src = static_cast<const T*>(p.src) + row * p.src_sr + col_block * F8Quantize::kBlock;
+      const int left = static_cast<int>(min(static_cast<long long>(F8Quantize::kBlock), p.cols - col_block * static_cast<long long>(F8Quantize::kBlock)));
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int at = (j * 8 + lane) * kPerLoad;
+        raw[i][j] = make_uint4(0, 0, 0, 0);
+        if (row < p.rows) {
+          if (at + kPerLoad <= left) {
+            raw[i][j] = __ldg(reinterpret_cast<const uint4*>(src + at));
+          } else if (at < left) {
+            T* x = reinterpret_cast<T*>(&raw[i][j]);
+            for (int e = 0; e < kPerLoad; ++e)
+              if (at + e < left) x[e] = src[at + e];
+          }
+        }
+      }
+      row += step_rows, col_block += step_cols;
+      if (col_block >= col_blocks) col_block -= col_blocks, ++row;
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      if (rows[i] >= p.rows) break;
+      float amax = f8_raw_amax<T>(raw[i][0]);
+#pragma unroll
+      for (int j = 1; j < kLoads; ++j) amax = fmaxf(amax, f8_raw_amax<T>(raw[i][j]));
+#pragma unroll
+      for (int offset = 4; offset > 0; offset >>= 1) amax = fmaxf(amax, __shfl_xor_sync(members, amax, offset));
+      amax = f8_bounded_amax(amax);
+      const float ratio = (lane == 7 ? amax : F8Quantize::kMax) / (lane == 7 ? F8Quantize::kMax : amax);
+      const float factor = __shfl_sync(members, ratio, 0, 8);
+      if (lane == 7) p.scale[rows[i] * p.scale_sr + cols[i] * p.scale_sc] = ratio;
+      uint8_t* dst = p.dst + rows[i] * p.dst_sr + cols[i] * static_cast<long long>(F8Quantize::kBlock);
+      const int left = static_cast<int>(min(static_cast<long long>(F8Quantize::kBlock), p.cols - cols[i] * static_cast<long long>(F8Quantize::kBlock)));
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int at = (j * 8 + lane) * kPerLoad;
+        f8_store_raw<T, true>(dst + at, raw[i][j], factor, left - at);
+      }
+    }
+  }
+}
+
+// 1 x 128 blocks of any strides: sixteen threads per block, eight elements each.
+template <typename T>
+__global__ void __launch_bounds__(256) f8_quantize_strided_kernel(const F8QuantizeArgs p) {
   const long long col_blocks = (p.cols + F8Quantize::kBlock - 1) / F8Quantize::kBlock;
   const long long total = p.rows * col_blocks;
   const int lane = threadIdx.x & 15;
@@ -89,31 +200,45 @@ __global__ void __launch_bounds__(256) f8_quantize_rows_kernel(const F8QuantizeA
     const long long row = block / col_blocks, col_block = block - row * col_blocks;
     const long long col = col_block * F8Quantize::kBlock + lane * 8;
     float x[8];
-    f8_load8<T, kVec>(static_cast<const T*>(p.src) + row * p.src_sr, p.src_sc, col, p.cols, x);
+    f8_load8<T, false>(static_cast<const T*>(p.src) + row * p.src_sr, p.src_sc, col, p.cols, x);
     float amax = f8_block_amax(x, 0.f);
     const unsigned members = 0xffffu << (threadIdx.x & 16);  // the other half of the warp may be done
 #pragma unroll
     for (int offset = 8; offset > 0; offset >>= 1) amax = fmaxf(amax, __shfl_xor_sync(members, amax, offset));
     amax = f8_bounded_amax(amax);
-    f8_store8<kVec>(p.dst + row * p.dst_sr, col, p.cols, x, F8Quantize::kMax / amax);
+    f8_store8<false>(p.dst + row * p.dst_sr, col, p.cols, x, F8Quantize::kMax / amax);
     if (lane == 0) p.scale[row * p.scale_sr + col_block * p.scale_sc] = amax / F8Quantize::kMax;
   }
 }
 
-// 128 x 128 blocks: one CTA per block holds it in registers between the maximum and the conversion.
+// 128 x 128 blocks: one CTA per block holds it, as loaded, in registers between the maximum and the conversion.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256) f8_quantize_tiles_kernel(const F8QuantizeArgs p) {
+  constexpr int kPerLoad = 16 / sizeof(T), kPieces = F8Quantize::kBlock / kPerLoad, kRowStep = 256 / kPieces, kLoads = F8Quantize::kBlock / kRowStep;
   __shared__ float warp_amax[8];
-  const long long row0 = blockIdx.y * static_cast<long long>(F8Quantize::kBlock) + (threadIdx.x >> 4);
-  const long long col = blockIdx.x * static_cast<long long>(F8Quantize::kBlock) + (threadIdx.x & 15) * 8;
-  float x[8][8];
+  const long long row0 = blockIdx.y * static_cast<long long>(F8Quantize::kBlock) + threadIdx.x / kPieces;
+  const long long col = blockIdx.x * static_cast<long long>(F8Quantize::kBlock) + threadIdx.x % kPieces * kPerLoad;
+  const int left = static_cast<int>(max(0ll, min(static_cast<long long>(kPerLoad), p.cols - col)));
+  uint4 raw[kLoads];
   float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const long long row = row0 + 16 * i;
-    f8_load8<T, kVec>(static_cast<const T*>(p.src) + (row < p.rows ? row : 0) * p.src_sr, p.src_sc, col, row < p.rows ? p.cols : 0, x[i]);
-    amax = f8_block_amax(x[i], amax);
+  for (int i = 0; i < kLoads; ++i) {
+    const long long row = row0 + kRowStep * i;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (row < p.rows) {
+      const T* src = static_cast<const T*>(p.src) + row * p.src_sr + col * p.src_sc;
+      if (kVec && left == kPerLoad) {
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(src));
+      } else {
+        T* x = reinterpret_cast<T*>(&raw[i]);
+#pragma unroll
+        for (int e = 0; e < kPerLoad; ++e)
+          if (e < left) x[e] = src[e * p.src_sc];
+      }
+    }
   }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) amax = fmaxf(amax, f8_raw_amax<T>(raw[i]));
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, offset));
   if ((threadIdx.x & 31) == 0) warp_amax[threadIdx.x >> 5] = amax;
@@ -123,9 +248,9 @@ __global__ void __launch_bounds__(256) f8_quantize_tiles_kernel(const F8Quantize
   amax = f8_bounded_amax(amax);
   const float factor = F8Quantize::kMax / amax;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const long long row = row0 + 16 * i;
-    if (row < p.rows) f8_store8<kVec>(p.dst + row * p.dst_sr, col, p.cols, x[i], factor);
+  for (int i = 0; i < kLoads; ++i) {
+    const long long row = row0 + kRowStep * i;
+    if (row < p.rows) f8_store_raw<T, kVec>(p.dst + row * p.dst_sr + col, raw[i], factor, left);
   }
   if (threadIdx.x == 0) p.scale[blockIdx.y * p.scale_sr + blockIdx.x * p.scale_sc] = amax / F8Quantize::kMax;
 }

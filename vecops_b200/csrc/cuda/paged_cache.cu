@@ -48,6 +48,7 @@ bool append_vectors(const VecopsB200CacheAppend& a) {
     if (s % 8 != 0) return false;
   for (const void* p : {a.q, a.k, a.v, static_cast<const void*>(a.q_out), static_cast<const void*>(a.k_cache), static_cast<const void*>(a.v_cache)})
     if (!decode_aligned(p, 16)) return false;
+  if (a.rotary > 0 && (!decode_aligned(a.cos_sin, 16) || a.cos_sin_stride % 4 != 0)) return false;
   return a.head_dim % 16 == 0 && a.rotary % 16 == 0;
 }
 
@@ -289,15 +290,18 @@ int32_t vecops_b200_cache_append(const VecopsB200CacheAppend* append, VecopsErro
   DecodeDevice device;
   rc = decode_enter(a.device_index, &device, error);
   if (rc != VECOPS_STATUS_OK) return rc;
-  const int64_t want = (a.tokens * per_token + 255) / 256;
-  const unsigned grid = static_cast<unsigned>(want < static_cast<int64_t>(device.sms) * 64 ? want : static_cast<int64_t>(device.sms) * 64);
+  const unsigned grid = static_cast<unsigned>(a.tokens < static_cast<int64_t>(device.sms) * 64 ? a.tokens : static_cast<int64_t>(device.sms) * 64);
+  // many tokens: small CTAs, whose lookups overlap with others' copies (8191 tokens: 38 us with 128 threads, 55 with 384); few: a token's
+  // copies all at once (64 tokens: 2.4 us with 384, 3.2 with 128)
+  const int64_t most = a.tokens >= static_cast<int64_t>(device.sms) * 8 ? 128 : kAppendThreads;
+  const unsigned threads = static_cast<unsigned>(per_token < most ? (per_token + 31) / 32 * 32 : most);
   cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
   if (a.dtype == VECOPS_DTYPE_BF16) {
-    if (vec) cache_append_kernel<__nv_bfloat16, true><<<grid, 256, 0, stream>>>(p);
-    else cache_append_kernel<__nv_bfloat16, false><<<grid, 256, 0, stream>>>(p);
+    if (vec) cache_append_kernel<__nv_bfloat16, true><<<grid, threads, 0, stream>>>(p);
+    else cache_append_kernel<__nv_bfloat16, false><<<grid, threads, 0, stream>>>(p);
   } else {
-    if (vec) cache_append_kernel<__half, true><<<grid, 256, 0, stream>>>(p);
-    else cache_append_kernel<__half, false><<<grid, 256, 0, stream>>>(p);
+    if (vec) cache_append_kernel<__half, true><<<grid, threads, 0, stream>>>(p);
+    else cache_append_kernel<__half, false><<<grid, threads, 0, stream>>>(p);
   }
   rc = decode_launched("cache_append", error);
   if (rc != VECOPS_STATUS_OK) return rc;

@@ -21,7 +21,7 @@ namespace vb200 {
 template <int kDim>
 struct SuffixSdpa {
   static constexpr int kWarps = 4, kThreads = 32 * kWarps;
-  static constexpr int kCtasPerSm = 3;
+  static constexpr int kCtasPerSm = 2;
   static constexpr int kRows = 16, kKeys = 16;
   static constexpr int kStages = 2;
   static constexpr int kRowBytes = kDim * 2;
