@@ -467,6 +467,131 @@ def test_prefix_attention_refuses(ops):
             ops.sdpa_shared_prefix(**{**good, **change})
 
 
+@pytest.mark.parametrize("batch,counts,hq,hkv,d", [(2100, None, 2, 1, 64), (700, [0, 1, 0, 2, 0, 0, 3], 4, 2, 64), (33, [16, 17, 1], 1, 1, 128), (5, [1, 2], 48, 1, 64)])
+def test_prefix_attention_of_many_and_of_uneven_sequences(ops, batch, counts, hq, hkv, d):
+    """More sequences than a warp has lanes, by far; empty ones between; items of many tokens; more query heads per key head than an
+    item has rows.  Lengths from nothing to two slices beside one long one."""
+    lengths = [(7 * i) % 33 for i in range(batch)]
+    lengths[batch // 2] = 900
+    counts = [1] * batch if counts is None else [counts[i % len(counts)] for i in range(batch)]
+    inputs = prefix_inputs(counts, lengths, 70, hq, hkv, d, 16, BF16, batch, ragged=max(counts) > 1)
+    check_prefix(ops, inputs)
+
+
+def test_prefix_attention_of_a_long_prefix_and_a_long_suffix(ops):
+    check_prefix(ops, prefix_inputs([1], [9000], 40000, 4, 1, 128, 64, BF16, 16, ragged=False))
+    check_prefix(ops, prefix_inputs([1] * 70, [5] * 70, 20000, 8, 2, 64, 128, F16, 17, ragged=False))
+
+
+@pytest.mark.parametrize("page", [3, 24, 48, 128, 384])
+def test_prefix_attention_of_page_sizes(ops, page):
+    # pages that end inside a slice of sixteen keys, or inside a tile of 128, and pages longer than a tile
+    check_prefix(ops, prefix_inputs([1, 1, 1], [50, 400, 129], 0, 8, 2, 64, page, BF16, page, ragged=False))
+    check_prefix(ops, prefix_inputs([2, 1, 3], [50, 400, 129], 777, 8, 2, 64, page, BF16, page))
+
+
+# ------------------------------------------------------------------------------------------------ the C ABI's own forms
+
+def run_record(function, record):
+    error = capi.ErrorBuffer()
+    error.raise_for(getattr(capi.library(), function)(capi.byref(record), capi.byref(error.record)))
+
+
+def f8_record(a, a_scale, b, b_scale, c, kernel):
+    r = capi.VecopsB200MatmulF8(struct_size=capi.ctypes.sizeof(capi.VecopsB200MatmulF8), kernel=kernel, m=a.shape[0], n=b.shape[0], k=a.shape[1],
+                                a=a.data_ptr(), a_stride_m=a.stride(0), a_stride_k=a.stride(1), a_scale=a_scale.data_ptr(),
+                                a_scale_stride_m=a_scale.stride(0), a_scale_stride_k=a_scale.stride(1), b=b.data_ptr(), b_stride_n=b.stride(0),
+                                b_stride_k=b.stride(1), b_scale=b_scale.data_ptr(), b_scale_stride_n=b_scale.stride(0),
+                                b_scale_stride_k=b_scale.stride(1), c=c.data_ptr(), c_stride_m=c.stride(0), c_stride_n=c.stride(1),
+                                c_dtype={BF16: capi.DTYPE_BF16, F16: capi.DTYPE_F16, F32: capi.DTYPE_F32}[c.dtype],
+                                stream=torch.cuda.current_stream().cuda_stream, device_index=0)
+    return r
+
+
+@pytest.mark.parametrize("kernel", [capi.F8_GENERIC, capi.F8_STREAM, capi.F8_TILED])
+@pytest.mark.parametrize("m,n,k", [(1, 130, 1024), (33, 700, 640), (128, 257, 2064)])
+def test_every_kernel_of_the_product(ops, m, n, k, kernel):
+    """The kernels on one problem, into rows with a gap behind them and into a transposed C; what lies between stays."""
+    a, a_scale, b, b_scale = product_operands(m, n, k, m + n)
+    want, magnitude = ref.matmul_f8(a, a_scale, b, b_scale)
+    for dtype in (BF16, F32):
+        for stored in (torch.full((m, n + 5), 7.0, dtype=dtype, device="cuda"), torch.full((n, m + 3), 7.0, dtype=dtype, device="cuda")):
+            c = stored[:, :n] if stored.shape[0] == m and stored.shape[1] == n + 5 else stored.t()[:m]
+            run_record("vecops_b200_matmul_f8_run", f8_record(a, a_scale, b, b_scale, c, kernel))
+            ref.assert_within(c, want, ref.matmul_f8_tolerance(want, magnitude, k, dtype))
+            rest = stored[:, n:] if c.stride(1) == 1 else stored[:, m:]
+            assert (rest == 7.0).all()
+
+
+def test_the_products_kernel_is_chosen_and_refused_by_rule(ops):
+    for m, n, k, kernel in ((1, 128, 128, capi.F8_STREAM), (128, 4096, 4096, capi.F8_STREAM), (129, 256, 512, capi.F8_TILED)):
+        a, a_scale, b, b_scale = product_operands(m, n, k, 1)
+        c = torch.empty(m, n, device="cuda")
+        chosen, error = capi.c_uint32(0), capi.ErrorBuffer()
+        error.raise_for(capi.library().vecops_b200_matmul_f8_select(capi.byref(f8_record(a, a_scale, b, b_scale, c, capi.F8_AUTO)), capi.byref(chosen), capi.byref(error.record)))
+        assert chosen.value == kernel
+    with pytest.raises(capi.VecopsB200Error) as info:
+        run_record("vecops_b200_matmul_f8_run", f8_record(a, a_scale, b, b_scale, c, capi.F8_STREAM))  # 129 rows
+    assert info.value.code == capi.NOT_APPLICABLE
+    odd = torch.zeros(130, 513, dtype=torch.uint8, device="cuda").view(E4M3)[:129, 1:]
+    chosen = capi.c_uint32(0)
+    error.raise_for(capi.library().vecops_b200_matmul_f8_select(capi.byref(f8_record(odd, a_scale, b, b_scale, c, capi.F8_AUTO)), capi.byref(chosen), capi.byref(error.record)))
+    assert chosen.value == capi.F8_GENERIC
+
+
+def append_record(q, k, v, q_out, k_cache, v_cache, slots, positions, table):
+    r = capi.VecopsB200CacheAppend(struct_size=capi.ctypes.sizeof(capi.VecopsB200CacheAppend), dtype=capi.DTYPE_BF16, tokens=k.shape[0], q_heads=q.shape[1] if q is not None else 0,
+                                   kv_heads=k.shape[1], head_dim=k.shape[2], pages=k_cache.shape[0], page_size=k_cache.shape[1], max_positions=table.shape[0],
+                                   rotary=table.shape[1], cos_sin_stride=table.stride(0), stream=torch.cuda.current_stream().cuda_stream, device_index=0)
+    for name, tensor in dict(q=q, k=k, v=v, q_out=q_out, k_cache=k_cache, v_cache=v_cache, slots=slots, positions=positions, cos_sin=table).items():
+        if tensor is not None:
+            setattr(r, name, tensor.data_ptr())
+    for name, tensor in dict(q=q, k=k, v=v, q_out=q_out).items():
+        if tensor is not None:
+            setattr(r, f"{name}_stride_token", tensor.stride(0)), setattr(r, f"{name}_stride_head", tensor.stride(1))
+    r.k_stride_page, r.k_stride_slot, r.k_cache_stride_head = k_cache.stride()[:3]
+    r.v_stride_page, r.v_stride_slot, r.v_cache_stride_head = v_cache.stride()[:3]
+    return r
+
+
+def test_append_in_place_and_without_queries(ops):
+    device = [t.cuda() for t in append_inputs(70, 8, 2, 64, 64, 16, 12, BF16, 30)]
+    q, k, v, k_cache, v_cache, slots, positions, table = device
+    want_k, want_v = k_cache.clone(), v_cache.clone()
+    want_q = ops.cache_append(q, k, v, want_k, want_v, slots, positions, table)
+    mine_k, mine_v, in_place = k_cache.clone(), v_cache.clone(), q.clone()
+    run_record("vecops_b200_cache_append", append_record(in_place, k, v, in_place, mine_k, mine_v, slots, positions, table))
+    assert torch.equal(in_place, want_q) and torch.equal(mine_k, want_k) and torch.equal(mine_v, want_v)
+    mine_k, mine_v = k_cache.clone(), v_cache.clone()
+    run_record("vecops_b200_cache_append", append_record(None, k, v, None, mine_k, mine_v, slots, positions, table))
+    assert torch.equal(mine_k, want_k) and torch.equal(mine_v, want_v)
+
+
+def test_prefix_attention_refuses_scratch_that_is_too_small(ops):
+    inputs = on_device(prefix_inputs([1] * 4, [30] * 4, 400, 8, 2, 64, 16, BF16, 31, ragged=False))
+    out = torch.full_like(inputs["q"], 7.0)
+    r = capi.VecopsB200PrefixAttention(struct_size=capi.ctypes.sizeof(capi.VecopsB200PrefixAttention), dtype=capi.DTYPE_BF16, tokens=4, batch=4, q_heads=8, kv_heads=2, head_dim=64,
+                                       pages=inputs["k_cache"].shape[0], page_size=16, prefix_len=400, table_stride=2, table_width=2, scale=0.125,
+                                       stream=torch.cuda.current_stream().cuda_stream, device_index=0)
+    for name in ("q", "k_cache", "v_cache", "prefix_pages", "page_table", "lengths"):
+        setattr(r, name, inputs[name].data_ptr())
+    r.out = out.data_ptr()
+    r.q_stride_token, r.q_stride_head, r.out_stride_token, r.out_stride_head = 512, 64, 512, 64
+    r.k_stride_page, r.k_stride_slot, r.k_stride_head = r.v_stride_page, r.v_stride_slot, r.v_stride_head = inputs["k_cache"].stride()[:3]
+    need, error = capi.c_uint64(0), capi.ErrorBuffer()
+    error.raise_for(capi.library().vecops_b200_prefix_sdpa_workspace(capi.byref(r), capi.byref(need), capi.byref(error.record)))
+    scratch = torch.empty(need.value + 256, dtype=torch.uint8, device="cuda")
+    for at, size in ((0, 0), (scratch.data_ptr(), need.value - 1), (scratch.data_ptr() + 8, need.value)):
+        r.workspace, r.workspace_size = at or None, size
+        with pytest.raises(capi.VecopsB200Error) as info:
+            run_record("vecops_b200_prefix_sdpa_run", r)
+        assert info.value.code == capi.INVALID_ARGUMENT and "scratch" in info.value.message
+    assert (out == 7.0).all()
+    r.workspace, r.workspace_size = scratch.data_ptr(), need.value
+    run_record("vecops_b200_prefix_sdpa_run", r)  # synchronous
+    assert torch.equal(out, ops.sdpa_shared_prefix(**inputs))
+
+
 # ------------------------------------------------------------------------------------------------ together, captured, on other streams
 
 def decode_step(ops, x, weights, k_cache, v_cache, tables, hq, hkv, d):

@@ -99,7 +99,7 @@ struct PrefixPlan {
   bool fast = false;  // the two kernels can address this call; the one-warp-per-row kernel serves the rest
   int dim = 0;        // head dims a kernel is built for: 64 or 128
   int both_rows = 0, row_blocks = 0, tiles = 0, tiles_per_chunk = 0, chunks = 0, records = 0;
-  int tokens_per_item = 1, group_tiles = 1, workers = 0;
+  int tokens_per_item = 1, group_tiles = 1, item_rows = 1, workers = 0;
   int64_t slots = 0, fragments = 0;
   uint64_t ml_at = 0, fragment_o_at = 0, fragment_ml_at = 0, sums_at = 0, total = 0;
 };
@@ -123,21 +123,24 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
     p.both_rows = rows > 128 ? 1 : 0;
     p.row_blocks = static_cast<int>(p.both_rows ? (rows + 255) / 256 : 1);
     p.tiles = static_cast<int>((a.prefix_len + 127) / 128);
-    // Cut the prefix so that the waves of work items are full: the cost of a cut is its waves times (tiles of an item + what an
-    // item costs besides, about two tiles: Q, the first loads, the records), and half a tile's worth per wave for the merge.
+    // Cut the prefix so that the waves of work items are full.  In units of a key tile's time (2 us with two row blocks): an item
+    // costs its tiles and about four more - Q, the first loads, the record it leaves - and a record of 10000 rows of 128 dims
+    // is a tile's worth of writing and merging.
     const int64_t base = a.kv_heads * p.row_blocks;
-    int64_t best = 0;
+    const double record_cost = static_cast<double>(a.kv_heads) * rows * p.dim / 1.28e6;
+    double best = 0;
     for (int chunks = 1; chunks <= p.tiles && chunks <= 128; ++chunks) {
       const int per_chunk = (p.tiles + chunks - 1) / chunks;
       const int used = (p.tiles + per_chunk - 1) / per_chunk;
       const int64_t waves = (base * used + sms - 1) / sms;
-      const int64_t cost = waves * (per_chunk + 2) * 2 + waves * (used > 1 ? 1 : 0);
+      const double cost = static_cast<double>(waves) * (per_chunk + 4) + record_cost * used;
       if (best == 0 || cost < best) best = cost, p.tiles_per_chunk = per_chunk, p.chunks = used;
     }
     p.records = p.both_rows ? p.chunks : 2 * p.chunks;
   }
   p.tokens_per_item = static_cast<int>(group <= 16 ? 16 / group : 1);
   p.group_tiles = static_cast<int>((group + 15) / 16);
+  p.item_rows = static_cast<int>(group >= 16 ? 16 : (a.query_starts == nullptr ? 1 : p.tokens_per_item) * group);
   p.slots = a.query_starts == nullptr ? a.batch : a.tokens / p.tokens_per_item + a.batch + 1;
   // warps for every slice the table could hold, up to what the SMs hold at once (slices are counted in 32 bits)
   const int64_t slices = (a.table_width * a.page_size + 15) / 16, columns = a.kv_heads * p.group_tiles;
@@ -159,8 +162,8 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
   const uint64_t record_rows = static_cast<uint64_t>(p.records) * a.kv_heads * rows;
   place(record_rows * p.dim * 4);
   p.ml_at = place(record_rows * 8);
-  p.fragment_o_at = place(static_cast<uint64_t>(p.fragments) * 16 * p.dim * 4);
-  p.fragment_ml_at = place(static_cast<uint64_t>(p.fragments) * 16 * 8);
+  p.fragment_o_at = place(static_cast<uint64_t>(p.fragments) * p.item_rows * p.dim * 4);
+  p.fragment_ml_at = place(static_cast<uint64_t>(p.fragments) * p.item_rows * 8);
   p.sums_at = place(static_cast<uint64_t>(p.slots + 1) * 4);
   return p;
 }
@@ -219,7 +222,7 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   SuffixSdpaArgs s{};
   s.a = args;
   s.rows = rows;
-  s.tokens_per_item = plan.tokens_per_item, s.group_tiles = plan.group_tiles;
+  s.tokens_per_item = plan.tokens_per_item, s.group_tiles = plan.group_tiles, s.item_rows = plan.item_rows;
   s.slots = static_cast<int>(plan.slots), s.workers = plan.workers;
   s.records = plan.records, s.partial_o = partial_o, s.partial_ml = partial_ml;
   char* base = static_cast<char*>(a.workspace);

@@ -42,8 +42,9 @@ struct SuffixSdpaArgs {
   int records;          // of the prefix kernel
   const float* partial_o;
   const float2* partial_ml;
-  float* fragment_o;    // [warp + item][16][kDim]
-  float2* fragment_ml;  // [warp + item][16]
+  int item_rows;        // rows an item has at most
+  float* fragment_o;    // [warp + item][item_rows][kDim]
+  float2* fragment_ml;  // [warp + item][item_rows]
   int* sums;            // [slot] weight of the slots before it, written where the slot has any; then [slots] the sum of all
 };
 
@@ -51,10 +52,9 @@ struct SuffixSdpaArgs {
 // query_starts[b] / tokens_per_item + b on: apart from each other, and found without a sum.
 constexpr int kItemWeight = 2;  // slices' worth of time that an item's lookups, queries and fragment take (measured: 2.5 us of 1 to 2 us each)
 
+// Suffix keys that token t sees of a sequence whose newest token is `newest`: of those the table has room for (fewer than 2^31).
 __device__ __forceinline__ int suffix_sees(const PrefixSdpaArgs& a, int length, int newest, int t) {
-  const long long capacity = static_cast<long long>(a.table_width) * a.page_size;
-  const long long seen = static_cast<long long>(length) - (newest - t);
-  return static_cast<int>(seen < 0 ? 0 : seen < capacity ? seen : capacity);
+  return max(0, min(length - (newest - t), a.table_width * a.page_size));
 }
 
 // The last sequence whose query_starts pass `before`, by a search 32 wide; the whole warp comes here.
@@ -282,25 +282,24 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
     for (int i = 1 - G::kStages; i < mine; ++i) {
       issue(i + G::kStages - 1);
       if (i < 0) {
-        // Q, behind the first copies: the A fragments of sixteen rows
-        {
-          const T* q_row[2];
-          bool there[2];
+        // Q, by way of the second stage, which is filled with keys only after this: the A fragments of sixteen rows
+        const uint32_t q_tile = ring + 2 * G::kTileBytes;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = h == 0 ? r_low : r_high;
-            there[h] = r < rows;
-            const int t = first + (there[h] ? r / heads : 0), head = kv * a.group + group0 + (there[h] ? r % heads : 0);
-            q_row[h] = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
-          }
-#pragma unroll
-          for (int ks = 0; ks < kDim / 16; ++ks)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int d = ks * 16 + (lane & 3) * 2 + (e >> 1) * 8;
-              q[ks][e] = there[e & 1] && d < a.head_dim ? *reinterpret_cast<const uint32_t*>(q_row[e & 1] + d) : 0u;
-            }
+        for (int step = 0; step < G::kRows / kRowsPerStep; ++step) {
+          const int row = step * kRowsPerStep + sub_row;
+          const bool there = row < rows && piece * 8 < a.head_dim;
+          const int t = first + (there ? row / heads : 0), head = kv * a.group + group0 + (there ? row % heads : 0);
+          cp_async_16(q_tile + row * G::kRowBytes + ((piece ^ (row & 7)) << 4), static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh + (there ? piece * 8 : 0), there ? 16 : 0);
         }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncwarp();
+#pragma unroll
+        for (int ks = 0; ks < kDim / 16; ++ks) {
+          const int row = lane & 15, at = ks * 2 + (lane >> 4);
+          ldmatrix_x4(q[ks], q_tile + row * G::kRowBytes + ((at ^ (row & 7)) << 4));
+        }
+        __syncwarp();
         continue;
       }
       cp_async_wait<G::kStages - 1>();
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
     __syncwarp();
 
     // ---- the fragment leaves
-    const size_t at = (static_cast<size_t>(worker) + static_cast<size_t>(slot) * columns + column) * G::kRows;
+    const size_t at = (static_cast<size_t>(worker) + static_cast<size_t>(slot) * columns + column) * p.item_rows;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = h == 0 ? r_low : r_high;
@@ -457,7 +456,7 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
       const int first_worker = worker_of(from + kItemWeight);  // (the item's extra weight lies before its slices)
       fragments = worker_of(from + weight - 1) - first_worker + 1;
       const int heads = min(16, a.group - in_group / 16 * 16);
-      first_fragment = (static_cast<size_t>(first_worker) + static_cast<size_t>(slot) * columns + column) * 16 + (t - first) * heads + in_group % 16;
+      first_fragment = (static_cast<size_t>(first_worker) + static_cast<size_t>(slot) * columns + column) * p.item_rows + (t - first) * heads + in_group % 16;
     }
   }
   // ---- this warp's share: eight partial results at a time, a lane per (m, l), four dims a lane, all their loads together
@@ -494,7 +493,7 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
   const size_t record_row = static_cast<size_t>(kv) * p.rows + static_cast<size_t>(t) * a.group + in_group;
   if (owned) {
     join(p.records, p.partial_ml + record_row, p.partial_o + record_row * kDim, static_cast<size_t>(a.kv_heads) * p.rows);
-    join(fragments, p.fragment_ml + first_fragment, p.fragment_o + first_fragment * kDim, 16);
+    join(fragments, p.fragment_ml + first_fragment, p.fragment_o + first_fragment * kDim, p.item_rows);
   }
 #pragma unroll
   for (int offset = 4; offset > 0; offset >>= 1) l += __shfl_xor_sync(0xffffffffu, l, offset);  // (the first eight lanes')
