@@ -164,7 +164,7 @@ typedef struct VecopsB200PrefixAttention {
   const int32_t* page_table;  /* [batch, table_width], contiguous rows */
   int64_t table_stride, table_width;
   const int32_t* lengths;     /* [batch] */
-  const int32_t* query_starts; /* [batch + 1], not decreasing, or NULL */
+  const int32_t* query_starts; /* [batch + 1], not decreasing, or NULL; what passes [0, tokens] counts as 0 or tokens */
   float scale;
   uint32_t flags;             /* VECOPS_B200_MATMUL_FLAG_ASYNC */
   void* workspace;            /* 256-byte aligned device scratch of vecops_b200_prefix_sdpa_workspace bytes */

@@ -109,6 +109,16 @@ def test_prefix_attention_refuses(library, changes):
     assert code_of("vecops_b200_prefix_sdpa_run", prefix_record(**changes))[0] == capi.INVALID_ARGUMENT
 
 
+def test_extents_past_the_grids_are_refused_or_left_to_the_simple_kernel(library):
+    code, message = code_of("vecops_b200_prefix_sdpa_run", prefix_record(tokens=1 << 30, batch=1 << 30, q_heads=1 << 15, kv_heads=1 << 15))
+    assert code == capi.INVALID_ARGUMENT and "too many" in message
+    need = ctypes.c_uint64(7)
+    many = prefix_record(tokens=1 << 23, batch=1 << 23, q_heads=8, kv_heads=1)  # 2^26 rows of one head: more blocks than a grid has
+    assert code_of("vecops_b200_prefix_sdpa_workspace", many, byref(need))[0] == capi.OK and need.value == 0
+    huge = 1 << 62  # (its double is negative)
+    assert code_of("vecops_b200_cache_append", append_record(kv_heads=huge))[0] == capi.INVALID_ARGUMENT
+
+
 ENTRIES = [("vecops_b200_quantize_blocks", quantize_record), ("vecops_b200_matmul_f8_run", matmul_record), ("vecops_b200_cache_append", append_record),
            ("vecops_b200_prefix_sdpa_run", prefix_record)]
 

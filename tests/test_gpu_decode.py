@@ -592,6 +592,37 @@ def test_prefix_attention_refuses_scratch_that_is_too_small(ops):
     assert torch.equal(out, ops.sdpa_shared_prefix(**inputs))
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("batch,prefix,hq,hkv,d", [(3, 900, 4, 2, 64), (40, 1000, 16, 2, 128)])
+def test_prefix_attention_of_large_scores(ops, dtype, sign, batch, prefix, hq, hkv, d):
+    # scores of +-(64 (d - 2) + 15) + r with r in eighths: exact in fp32, thousands away from zero and a few apart
+    inputs = prefix_inputs([1] * batch, [40] * batch, prefix, hq, hkv, d, 16, dtype, 41, ragged=False, scale=1.0)
+    inputs["q"][:], inputs["k_cache"][:] = 8.0 * sign, 8.0
+    inputs["q"][..., d // 2] = 1.0
+    inputs["q"][..., d // 2 + 1], inputs["k_cache"][..., d // 2 + 1] = sign, 15.0
+    inputs["k_cache"][..., d // 2] = (torch.randint(-24, 25, inputs["k_cache"].shape[:3], generator=generator(42)) / 8).to(dtype)
+    out = ops.sdpa_shared_prefix(**on_device(inputs))
+    want, _ = ref.prefix_attention(**inputs)
+    size, _ = ref.prefix_attention(**{**inputs, "v_cache": inputs["v_cache"].abs()})
+    # In units of log2(e) a score is below 2^14: a product with the scale is off by 2^-11 (a key's own, or the maximum's it
+    # is measured from), so a weight by 2 of them and the weights' sum by as much; p and the result are rounded to the type
+    step = ref.half_step(dtype)
+    relative = 4 * math.log(2) * 2.0 ** -11 + step + 2.0 ** -16
+    tiny = 2.0 ** -25 * (prefix + 41) * 5 if dtype == F16 else 0.0
+    ref.assert_within(out, want, 1.05 * (2 * relative * size + step * want.abs()) + tiny)
+
+
+def test_prefix_attention_ignores_query_tokens_that_do_not_exist(ops):
+    # starts before the first token and behind the last: the tokens there are nobody's
+    for d in (64, 80, 72, 256):
+        inputs = prefix_inputs([2, 3, 1], [40, 50, 20], 200, 8, 2, d, 16, BF16, 43)
+        inside = dict(inputs, query_starts=torch.tensor([0, 2, 5, 6], dtype=torch.int32))
+        whole = ops.sdpa_shared_prefix(**on_device(inside))
+        outside = on_device(dict(inputs, query_starts=torch.tensor([-3, 2, 5, 9], dtype=torch.int32)))
+        assert torch.equal(ops.sdpa_shared_prefix(**outside), whole), d
+
+
 # ------------------------------------------------------------------------------------------------ together, captured, on other streams
 
 def decode_step(ops, x, weights, k_cache, v_cache, tables, hq, hkv, d):

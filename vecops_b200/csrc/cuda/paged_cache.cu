@@ -19,7 +19,7 @@ bool sixteen_bit(uint32_t dtype) { return dtype == VECOPS_DTYPE_BF16 || dtype ==
 int32_t check_append(const VecopsB200CacheAppend& a, VecopsError* error) {
   if (!sixteen_bit(a.dtype)) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "cache_append serves bf16 and f16, not dtype %u", a.dtype);
   if (a.tokens < 0 || a.q_heads < 0 || a.kv_heads < 0 || a.head_dim < 0 || a.pages < 0 || a.page_size < 0 || a.tokens >= (INT64_C(1) << 31) ||
-      a.q_heads + 2 * a.kv_heads > (1 << 20) || a.head_dim > (1 << 10) || a.page_size >= (INT64_C(1) << 31))
+      a.q_heads > (1 << 20) || a.kv_heads > (1 << 20) || a.q_heads + 2 * a.kv_heads > (1 << 20) || a.head_dim > (1 << 10) || a.page_size >= (INT64_C(1) << 31))
     return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "cache_append: extent out of range");
   if (a.pages > 0 && a.page_size > INT64_MAX / a.pages) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "cache_append: the cache has too many slots");
   if (a.rotary < 0 || a.rotary > a.head_dim || a.rotary % 2 != 0)
@@ -60,6 +60,7 @@ int32_t check_prefix(const VecopsB200PrefixAttention& a, VecopsError* error) {
     return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: extent out of range");
   if (a.q_heads < 1 || a.kv_heads < 1 || a.q_heads % a.kv_heads != 0 || a.q_heads > 65535)
     return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: %lld query heads over %lld key heads", (long long)a.q_heads, (long long)a.kv_heads);
+  if (a.tokens * a.q_heads > 4 * INT64_C(0x7fffffff)) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
   if (a.head_dim < 1 || a.head_dim > 256) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: head_dim must be 1..256, not %lld", (long long)a.head_dim);
   if (a.table_width * a.page_size >= limit - a.prefix_len)
     return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: a sequence could have 2^31 keys");
@@ -115,7 +116,8 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
            rows_ok(a.q, a.tokens, a.q_stride_token, a.q_heads, a.q_stride_head, 1, 0) && rows_ok(a.out, a.tokens, a.out_stride_token, a.q_heads, a.out_stride_head, 1, 0) &&
            rows_ok(a.k_cache, a.pages, a.k_stride_page, a.page_size, a.k_stride_slot, a.kv_heads, a.k_stride_head) &&
            rows_ok(a.v_cache, a.pages, a.v_stride_page, a.page_size, a.v_stride_slot, a.kv_heads, a.v_stride_head) &&
-           a.tokens * (a.q_heads / a.kv_heads) < (INT64_C(1) << 31) - 256 && a.kv_heads <= 65535 && a.batch < (1 << 24) && a.tokens < (1 << 24);
+           a.tokens * (a.q_heads / a.kv_heads) <= INT64_C(256) * 65535 &&  // (row blocks are a grid's third dimension)
+           a.kv_heads <= 65535 && a.batch < (1 << 24) && a.tokens < (1 << 24);
   if (!p.fast) return p;
   p.dim = a.head_dim <= 64 ? 64 : 128;
   const int64_t group = a.q_heads / a.kv_heads, rows = a.tokens * group;
@@ -240,7 +242,6 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   const int64_t out_rows = a.tokens * a.q_heads;
   const bool shared_rows = out_rows <= static_cast<int64_t>(device.sms) * 4;
   const int64_t blocks = shared_rows ? out_rows : (out_rows + 3) / 4;
-  if (blocks > 0x7fffffff) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
   config.gridDim = dim3(static_cast<unsigned>(blocks));
   config.blockDim = dim3(128);
   config.dynamicSmemBytes = 0;
@@ -252,7 +253,6 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
 template <typename T>
 int32_t run_prefix_generic(const VecopsB200PrefixAttention& a, VecopsError* error) {
   const int64_t blocks = (a.tokens * a.q_heads + 7) / 8;
-  if (blocks >= (INT64_C(1) << 31)) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: too many query rows");
   prefix_sdpa_generic_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(a.stream)>>>(prefix_args(a));
   return decode_launched("prefix_sdpa (generic)", error);
 }

@@ -46,10 +46,11 @@ struct PrefixTc {
   static constexpr int kMaskOffset = kSpace;
   static constexpr int kMaskSlots = 16;                  // per key tile: which of its pages lie outside the cache
   static constexpr int kExchangeOffset = kMaskOffset + kMaskSlots * 4;
-  static constexpr int kExchangeBytes = 2 * 2 * 128 * 2;  // [group][half of the row][row] bf16
+  static constexpr int kExchangeBytes = 2 * 2 * 128 * 4;  // [group][half of the row][row] fp32
   static constexpr int kBarrierOffset = kExchangeOffset + kExchangeBytes;
   static constexpr int kBarriers = 2 * kMostSteps + 5;
-  static constexpr int kSmemBytes = kBarrierOffset + kBarriers * 8 + 8 + 1024;
+  static constexpr int kAlign = 256;                     // of dynamic shared memory; the tiles' swizzle wants 1024
+  static constexpr int kSmemBytes = kBarrierOffset + kBarriers * 8 + 8 + 1024 - kAlign;
   static constexpr int kFirstSoftmaxWarp = 4, kGroupWarps = 8;
   static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + 2 * kGroupWarps);
   static constexpr int kPolynomialPairs = 4;             // of 16 pairs of exponentials, those computed beside the special-function units
@@ -128,7 +129,7 @@ template <typename T, int kDim>
 __global__ void __launch_bounds__(PrefixTc<kDim>::kThreads, 1)
 prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixTcArgs p) {
   using G = PrefixTc<kDim>;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(PrefixTc<128>::kAlign) uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t full_bar = smem_base + G::kBarrierOffset;  // [steps] a step's tiles landed       (TMA -> MMA)
@@ -326,7 +327,7 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const int row = row0 + (p.both_rows ? g * G::kRows : 0) + row_local;
     const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + g * 256;
     const uint32_t my_scores = my_tmem + half * 64, my_o = my_tmem + 128 + half * (kDim / 2);
-    __nv_bfloat16* exchange = reinterpret_cast<__nv_bfloat16*>(smem_gen + G::kExchangeOffset) + g * 256 + row_local;  // [half][row]
+    volatile float* exchange = reinterpret_cast<volatile float*>(smem_gen + G::kExchangeOffset) + g * 256 + row_local;  // [half][row]
     auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quarter) : "memory"); };         // the two warps of a quarter's rows
     const float signed_scale = p.a.scale * 1.4426950408889634f;  // scores in units of log2(e)
     const float scale = signed_scale == 0.f ? 1.f : fabsf(signed_scale);
@@ -375,11 +376,10 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           highest = fmaxf(top[0], top[1]);
         }
       }
-      // The two halves agree on a maximum rounded to 16 bits: any m near it serves, as long as it is the same for the row.
-      const __nv_bfloat16 rounded = __float2bfloat16_rn(highest);
-      exchange[half * 128] = rounded;
+      // The two halves agree on the row's maximum.  (In 32 bits: rounded to 16, one of thousands is off by tens, and p past what fp16 holds.)
+      exchange[half * 128] = highest;
       meet();
-      const float tile_max = fmaxf(__bfloat162float(rounded), __bfloat162float(exchange[(half ^ 1) * 128])) * scale;
+      const float tile_max = fmaxf(highest, exchange[(half ^ 1) * 128]) * scale;
       const bool moves = turn == 0 || tile_max > m + 8.f;
       if (turn == 0) {
         m = tile_max;
@@ -461,11 +461,11 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       }
     }
-    // the row's sum: the second half's goes to the first through the exchange, whose 256 maxima of this group make 128 floats
-    float* sum_of = reinterpret_cast<float*>(smem_gen + G::kExchangeOffset) + g * 128 + row_local;
-    if (half == 1) *sum_of = l;
+    // the row's sum: the second half's goes to the first through the place of its own maxima, which the first has read: its
+    // probabilities of the last tile have arrived
+    if (half == 1) exchange[128] = l;
     meet();
-    if (half == 0) l += *sum_of;
+    if (half == 0) l += exchange[128];
     if (half == 0 && row < p.rows) __stcg(p.partial_ml + at, make_float2(turn > 0 && ok ? m : -INFINITY, turn > 0 && ok ? l : 0.f));
   }
 

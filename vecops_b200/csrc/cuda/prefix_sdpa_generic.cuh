@@ -42,7 +42,7 @@ __device__ __forceinline__ bool prefix_token(const PrefixSdpaArgs& p, int t, int
       else high = middle;
     }
     sequence = low;
-    newer = p.query_starts[low + 1] - 1 - t;
+    newer = min(p.tokens, p.query_starts[low + 1]) - 1 - t;
   }
   const int length = p.lengths[sequence];
   if (length < 0) return false;

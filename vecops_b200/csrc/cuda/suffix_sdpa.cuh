@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
   if (a.query_starts != nullptr) {
     owned = there && a.batch > 0 && t >= a.query_starts[0] && t < a.query_starts[a.batch];
     sequence = owned ? suffix_search(a.batch, [&](int b) { return a.query_starts[b] <= t; }) : 0;  // (the same for the warp)
-    if (owned) start = a.query_starts[sequence], newest = a.query_starts[sequence + 1] - 1;
+    if (owned) start = max(0, a.query_starts[sequence]), newest = min(a.tokens, a.query_starts[sequence + 1]) - 1;
   }
   const int length = owned ? a.lengths[sequence] : -1;
   owned = owned && length >= 0;
