@@ -5,7 +5,8 @@
  * These stand next to the quantised matmul rows and the attention caller of matmul_cuda.h and follow its rules: all
  * pointers are DEVICE pointers on `device_index`, strides count elements, nothing allocates device memory, errors come
  * back as VecopsStatusCode with a message, calls are synchronous unless VECOPS_B200_MATMUL_FLAG_ASYNC is set, and there
- * is no CPU fallback.  The reference has no counterpart of these operators.
+ * is no CPU fallback.  The first call on a device sets it up; make it before any stream capture begins.  Calls whose outputs
+ * and scratch are apart may run at once, on any streams.  The reference has no counterpart of these operators.
  *
  *     vecops_b200_quantize_blocks     x -> e4m3 values and an fp32 scale per 1 x 128 or 128 x 128 block
  *     vecops_b200_matmul_f8_run       C = sum over 128-blocks of K of a_scale * b_scale * (A_block . B_block^T)

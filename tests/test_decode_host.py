@@ -52,7 +52,10 @@ def matmul_record(**changes):
 
 def append_record(**changes):
     r = capi.VecopsB200CacheAppend(struct_size=ctypes.sizeof(capi.VecopsB200CacheAppend), dtype=capi.DTYPE_BF16, tokens=4, q_heads=8, kv_heads=2,
-                                   head_dim=64, pages=10, page_size=16, max_positions=100, rotary=64, cos_sin_stride=64, device_index=-1)
+                                   head_dim=64, pages=10, page_size=16, max_positions=100, rotary=64, cos_sin_stride=64, device_index=-1,
+                                   q_stride_token=512, q_stride_head=64, k_stride_token=128, k_stride_head=64, v_stride_token=128, v_stride_head=64,
+                                   q_out_stride_token=512, q_out_stride_head=64, k_stride_page=2048, k_stride_slot=128, k_cache_stride_head=64,
+                                   v_stride_page=2048, v_stride_slot=128, v_cache_stride_head=64)
     for key in ("q", "k", "v", "q_out", "k_cache", "v_cache", "slots", "positions", "cos_sin"):
         setattr(r, key, SOMEWHERE)
     for key, value in changes.items():
@@ -107,6 +110,18 @@ def test_prefix_attention_refuses(library, changes):
     need = ctypes.c_uint64(0)
     assert code_of("vecops_b200_prefix_sdpa_workspace", prefix_record(**changes), byref(need))[0] == capi.INVALID_ARGUMENT
     assert code_of("vecops_b200_prefix_sdpa_run", prefix_record(**changes))[0] == capi.INVALID_ARGUMENT
+
+
+def test_outputs_that_share_memory_are_refused(library):
+    for changes in (dict(scale_stride_row=0), dict(scale_stride_col=0)):
+        code, message = code_of("vecops_b200_quantize_blocks", quantize_record(**changes))
+        assert code == capi.INVALID_ARGUMENT and "share memory" in message, changes
+    for name in ("k_stride_page", "k_stride_slot", "k_cache_stride_head", "v_stride_page", "v_stride_slot", "v_cache_stride_head", "q_out_stride_token", "q_out_stride_head"):
+        code, message = code_of("vecops_b200_cache_append", append_record(**{name: 0}))
+        assert code == capi.INVALID_ARGUMENT and "share memory" in message, name
+    for name in ("out_stride_token", "out_stride_head"):
+        code, message = code_of("vecops_b200_prefix_sdpa_run", prefix_record(**{name: 0}))
+        assert code == capi.INVALID_ARGUMENT and "share memory" in message, name
 
 
 def test_extents_past_the_grids_are_refused_or_left_to_the_simple_kernel(library):

@@ -744,3 +744,37 @@ def test_steps_on_two_streams_at_once(ops):
         for result in [*results[i], graphs[i][1]]:
             for mine, theirs in zip(result, state[-1]):
                 assert torch.equal(mine, theirs)
+
+
+def test_branches_of_a_captured_graph_join(ops):
+    # products on one branch, attention on the other, a product behind both: launches that wait for more than one kernel
+    inputs = on_device(prefix_inputs([1] * 6, [40, 3, 0, 17, 64, 9], 700, 8, 2, 64, 16, BF16, 51, ragged=False))
+    g = generator(52)
+    x = torch.randn(6, 512, generator=g).to(BF16).cuda()
+    w, w_scale = ops.quantize_blocks(torch.randn(512, 512, generator=g).to(BF16).cuda(), 128)
+    side = torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            y = ops.matmul_f8_blocks(*ops.quantize_blocks(x, 1), w, w_scale, BF16)
+        o = ops.sdpa_shared_prefix(**inputs)
+        here.wait_stream(side)
+        z = ops.matmul_f8_blocks(*ops.quantize_blocks(o.view(6, 512), 1), w, w_scale, BF16)
+        t = ops.sdpa_shared_prefix(**dict(inputs, q=z.view(6, 8, 64)))
+        return y, o, z, t
+
+    want = [r.clone() for r in run()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        for r in got:
+            r.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for r, e in zip(got, want):
+            assert torch.equal(r, e)
+    del graph

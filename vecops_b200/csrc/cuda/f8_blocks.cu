@@ -249,6 +249,8 @@ int32_t vecops_b200_quantize_blocks(const VecopsB200QuantizeBlocks* quantize, Ve
   if (q.rows > 1 && q.dst_stride_row < q.cols)
     return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "quantize_blocks: rows of dst overlap (pitch %lld for %lld columns)",
                      (long long)q.dst_stride_row, (long long)q.cols);
+  if ((q.rows > q.block_rows && q.scale_stride_row == 0) || (q.cols > 128 && q.scale_stride_col == 0))
+    return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "quantize_blocks: scales share memory");
   if (q.src == nullptr || q.dst == nullptr || q.scale == nullptr) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "quantize_blocks: null pointer");
   const DeviceRestore restore;
   DecodeDevice device;

@@ -31,6 +31,10 @@ int32_t check_append(const VecopsB200CacheAppend& a, VecopsError* error) {
   for (int64_t s : strides)
     if (s < 0) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "cache_append: negative stride or table size");
   if (a.tokens == 0 || a.head_dim == 0) return VECOPS_STATUS_OK;
+  auto shares = [&](int64_t page, int64_t slot, int64_t head) { return (a.pages > 1 && page == 0) || (a.page_size > 1 && slot == 0) || (a.kv_heads > 1 && head == 0); };
+  if (shares(a.k_stride_page, a.k_stride_slot, a.k_cache_stride_head) || shares(a.v_stride_page, a.v_stride_slot, a.v_cache_stride_head) ||
+      (a.q != nullptr && ((a.tokens > 1 && a.q_out_stride_token == 0) || (a.q_heads > 1 && a.q_out_stride_head == 0))))
+    return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "cache_append: rows of the cache or of q_out share memory");
   if ((a.q == nullptr) != (a.q_out == nullptr) && a.q_heads > 0)
     return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "cache_append: q and q_out come together");
   if (a.slots == nullptr || (a.kv_heads > 0 && (a.k == nullptr || a.v == nullptr)) ||
@@ -72,6 +76,8 @@ int32_t check_prefix(const VecopsB200PrefixAttention& a, VecopsError* error) {
   for (int64_t s : strides)
     if (s < 0) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: negative stride");
   if (a.tokens == 0) return VECOPS_STATUS_OK;
+  if ((a.tokens > 1 && a.out_stride_token == 0) || (a.q_heads > 1 && a.out_stride_head == 0))
+    return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: rows of out share memory");
   if (a.q == nullptr || a.out == nullptr || (a.pages > 0 && (a.k_cache == nullptr || a.v_cache == nullptr)) || (a.batch > 0 && a.lengths == nullptr) ||
       (a.prefix_len > 0 && a.prefix_pages == nullptr) || (a.batch > 0 && a.table_width > 0 && a.page_table == nullptr))
     return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa: null pointer");
