@@ -4,12 +4,14 @@
 //
 // A block's scales apply to its sum over 128 k, so every 128-k step of the main loop is an accumulation of its own, which
 // eight warps read back from tensor memory and add, scaled, to totals in registers while the tensor cores work on the next.
-// Four MMAs of 256 columns take 512 cycles; the round trip MMA -> commit -> read-back -> arrival -> MMA of an
-// accumulator is what keeps the kernel from that rate, as tensor memory holds two of them.  (Four accumulators of 128
-// columns hide it better, but an MMA of 128 columns takes 80 cycles, not 64, and measured 12 % slower; shared memory,
-// which the MMAs and the arriving tiles keep busy, makes every barrier slow, too.)  Roles, per CTA:
+// Four MMAs of 256 columns take 512 cycles; a step of the totals' loop takes some 750: the wait for its sums, 340 for reading
+// them back while the MMAs of the other accumulator work on the same tensor memory, 256 of multiply-adds.  That loop is what
+// bounds the kernel: without its multiply-adds it reached 2.7 PFLOP/s, with them 4096 x 14336 x 4096 takes 209 us, 2.3
+// PFLOP/s.  (Tensor memory holds two accumulators of 256 columns.  Four of 128 hide the round trip better, but an MMA of 128
+// columns takes 80 cycles, not 64, and measured 12 % slower; sixteen warps of totals, wider reads, reads across steps and
+// scales fetched a step ahead measured slower or the same.)  512 x 4096 x 14336, cut into slices of K: 33 us.  Roles, per CTA:
 //   warp 0      TMA: its 128 rows of A and its 128 of the tile's 256 rows of B per step, a ring of kStages
-//   warp 1      (leader CTA) issues tcgen05.mma.cta_group::2, M = 256, N = 128, four of 32 k per accumulator
+//   warp 1      (leader CTA) issues tcgen05.mma.cta_group::2, M = 256, N = 256, four of 32 k per accumulator
 //   warps 2-3   fetch the scales into a ring in shared memory, up to 32 steps ahead (fetched by the totals' own threads, 32
 //               rows a warp and each in a line of its own, they took as long as the product itself)
 //   warps 4-11  totals - a thread owns one row and 128 columns of C, all of one weight block: one factor sa * sb per step
@@ -26,7 +28,7 @@ struct F8Tiled {
   static constexpr int kTile = 256;
   static constexpr int kOperandBytes = 128 * 128;  // 128 rows x 128 bytes of A, and as much of B
   static constexpr int kStageBytes = 2 * kOperandBytes;
-  static constexpr int kStages = 6;
+  static constexpr int kStages = 5;
   static constexpr int kAccumulators = 2;
   static constexpr int kTotalWarps = 8;
   static constexpr int kFirstTotalWarp = 4;  // register shares are per warpgroup
@@ -34,8 +36,10 @@ struct F8Tiled {
   // 384 threads x 168 registers at launch; the totals take what the other warpgroup gives up: (56 + 2 x 224) x 128 = 168 x 384
   static constexpr int kFewRegisters = 56, kManyRegisters = 224;
   static constexpr int kOutRows = 16;                        // rows of C a warp stages at a time, 128 bytes of each
+  // ... and how many such pieces may be on their way (one, with the room in a sixth stage, took 2 % longer)
+  static constexpr int kOutBuffers = 3;
   static constexpr int kOutOffset = kStages * kStageBytes;
-  static constexpr int kOutBytes = kTotalWarps * kOutRows * 128;
+  static constexpr int kOutBytes = kTotalWarps * kOutBuffers * kOutRows * 128;
   static constexpr int kScaleSteps = 4, kScaleSlots = 8;     // a slot holds four steps' scales of the tile's 128 rows and two weight blocks
   static constexpr int kScaleOffset = kOutOffset + kOutBytes;
   static constexpr int kSlotFloats = kScaleSteps * (128 + 2);
@@ -218,7 +222,8 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kManyRegisters));
     const int quarter = warp & 3, half = (warp - G::kFirstTotalWarp) >> 2;
-    const uint32_t out_buf = smem_base + G::kOutOffset + (warp - G::kFirstTotalWarp) * (G::kOutRows * 128);
+    const uint32_t out_ring = smem_base + G::kOutOffset + (warp - G::kFirstTotalWarp) * (G::kOutBuffers * G::kOutRows * 128);
+    int out_at = 0;
     const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
     int stage = 0, acc = 0, slot = 0;
     uint32_t phase = 0, slot_phase = 0;
@@ -228,6 +233,7 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       tile_coords(tile, tiles_m, tiles_n, raster_group, tm, tn);
       const int row0 = tm * G::kTile + static_cast<int>(rank) * 128 + quarter * 32;
       const int col0 = tn * G::kTile + half * 128;
+      bool early = false;  // the next step's sums are ready: asked under this step's last multiplications (asked when needed, it took some 180 cycles)
       float2 total[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) total[j] = make_float2(0.f, 0.f);
@@ -249,7 +255,7 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const float s = factor[0];
 #pragma unroll
         for (int g = 0; g + 1 < G::kScaleSteps; ++g) factor[g] = factor[g + 1];
-        if (!__all_sync(0xffffffffu, mbar_wait(done_bar + 8 * stage, phase, abort_flag))) {
+        if (!__all_sync(0xffffffffu, early) && !__all_sync(0xffffffffu, mbar_wait(done_bar + 8 * stage, phase, abort_flag))) {
           if (lane == 0) give_up(kStatusEpilogueWait);
           ok = false;
           break;
@@ -261,6 +267,7 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
         for (int chunk = 0; chunk < 8; ++chunk) {
           tmem_load_wait();
+          if (chunk == 7) early = mbar_test_wait(done_bar + 8 * (stage + 1 == G::kStages ? 0 : stage + 1), stage + 1 == G::kStages ? phase ^ 1u : phase);
           if (chunk + 1 < 8) {
             tmem_load_32x16(taddr + 16 * (chunk + 1), v[(chunk + 1) & 1]);
           } else {
@@ -306,8 +313,10 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           }
 #pragma unroll
           for (int part = 0; part < 32 / G::kOutRows; ++part) {
-            if (lane == 0) tma_store_wait_read<0>();  // the rows before these have left the buffer
+            if (lane == 0) tma_store_wait_read<G::kOutBuffers - 1>();  // what was in this buffer has left it
             __syncwarp();
+            const uint32_t out_buf = out_ring + out_at * (G::kOutRows * 128);
+            if (++out_at == G::kOutBuffers) out_at = 0;
             if (lane / G::kOutRows == part) {
 #pragma unroll
               for (int piece = 0; piece < 8; ++piece) {
