@@ -137,12 +137,13 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
     const int64_t base = a.kv_heads * p.row_blocks;
     const double record_cost = static_cast<double>(a.kv_heads) * rows * p.dim / 1.28e6;
     double best = 0;
-    for (int chunks = 1; chunks <= p.tiles && chunks <= 128; ++chunks) {
-      const int per_chunk = (p.tiles + chunks - 1) / chunks;
-      const int used = (p.tiles + per_chunk - 1) / per_chunk;
+    for (int per_chunk = p.tiles, used = 1; used <= 128;) {
       const int64_t waves = (base * used + sms - 1) / sms;
       const double cost = static_cast<double>(waves) * (per_chunk + 4) + record_cost * used;
       if (best == 0 || cost < best) best = cost, p.tiles_per_chunk = per_chunk, p.chunks = used;
+      if (per_chunk == 1) break;
+      used = (p.tiles + per_chunk - 2) / (per_chunk - 1);  // the fewest chunks that are shorter (each length once: the rest cut alike)
+      per_chunk = (p.tiles + used - 1) / used;
     }
     p.records = p.both_rows ? p.chunks : 2 * p.chunks;
   }
