@@ -76,6 +76,16 @@ def test_quantizer_reads_strided_and_unaligned_sources(ops):
             assert same_bits(q.cpu(), want) and torch.equal(scale.cpu(), want_scale)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantizer_of_many_rows_off_boundaries(ops, dtype, block_rows):
+    # more blocks than the grid's warps have at once, every row's start at another offset, the last block ragged
+    x = torch.randn(1500, 1999, generator=generator(5)).to(dtype)
+    want, want_scale = ref.quantize(x, block_rows)
+    q, scale = ops.quantize_blocks(x.cuda(), block_rows)
+    assert torch.equal(scale.cpu(), want_scale) and same_bits(q.cpu(), want)
+
+
 def test_quantizer_of_nothing(ops):
     for shape in ((0, 128), (4, 0)):
         q, scale = ops.quantize_blocks(torch.empty(shape, dtype=BF16, device="cuda"))
@@ -537,6 +547,24 @@ def test_the_products_kernel_is_chosen_and_refused_by_rule(ops):
     chosen = capi.c_uint32(0)
     error.raise_for(capi.library().vecops_b200_matmul_f8_select(capi.byref(f8_record(odd, a_scale, b, b_scale, c, capi.F8_AUTO)), capi.byref(chosen), capi.byref(error.record)))
     assert chosen.value == capi.F8_GENERIC
+
+
+@pytest.mark.parametrize("kernel", [capi.F8_STREAM, capi.F8_TILED, capi.F8_GENERIC])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("row,col,start", [(1, 120, 0), (301, 1, 1), (900, 2, 3), (304, 1, 0)])
+def test_product_stores_into_any_strides(ops, kernel, dtype, row, col, start):
+    m, n, k = 117, 299, 400
+    a, a_scale, b, b_scale = product_operands(m, n, k, 21)
+    whole = torch.full((300 * 120 + 900 * 120 + 8,), -3.0, dtype=dtype, device="cuda")
+    before = whole.clone()
+    c = whole.as_strided((m, n), (row, col), start)
+    r = f8_record(a, a_scale, b, b_scale, c, kernel)
+    r.c_dtype = {BF16: capi.DTYPE_BF16, F16: capi.DTYPE_F16, F32: capi.DTYPE_F32}[dtype]
+    run_record("vecops_b200_matmul_f8_run", r)
+    want, magnitude = ref.matmul_f8(a, a_scale, b, b_scale)
+    ref.assert_within(c, want, ref.matmul_f8_tolerance(want, magnitude, k, dtype))
+    before.as_strided((m, n), (row, col), start).copy_(c)
+    assert torch.equal(whole, before)  # and nothing beside them
 
 
 def append_record(q, k, v, q_out, k_cache, v_cache, slots, positions, table):

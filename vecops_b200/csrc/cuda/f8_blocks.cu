@@ -20,10 +20,11 @@ template <typename T>
 int32_t quantize_typed(const VecopsB200QuantizeBlocks& q, int sms, VecopsError* error) {
   F8QuantizeArgs p{q.src, q.src_stride_row, q.src_stride_col, static_cast<uint8_t*>(q.dst), q.dst_stride_row,
                    q.scale, q.scale_stride_row, q.scale_stride_col, q.rows, q.cols};
-  // sixteen bytes per load and eight per store where every row allows it
-  const bool vec = (q.src_stride_col == 1 || q.cols == 1) && decode_aligned(q.src, 16) &&
-                   (q.rows == 1 || q.src_stride_row * static_cast<int64_t>(sizeof(T)) % 16 == 0) && decode_aligned(q.dst, 8) &&
-                   (q.rows == 1 || q.dst_stride_row % 8 == 0);
+  // sixteen bytes per load and eight per store where every row allows it; four elements a lane where the rows of src are only contiguous
+  const bool rows_ok = q.src_stride_col == 1 || q.cols == 1;
+  const bool vec = rows_ok && decode_aligned(q.src, 16) && (q.rows == 1 || q.src_stride_row * static_cast<int64_t>(sizeof(T)) % 16 == 0) &&
+                   decode_aligned(q.dst, 8) && (q.rows == 1 || q.dst_stride_row % 8 == 0);
+  const bool unaligned = !vec && rows_ok && decode_aligned(q.dst, 4) && (q.rows == 1 || q.dst_stride_row % 4 == 0);
   cudaStream_t stream = static_cast<cudaStream_t>(q.stream);
   const int64_t col_blocks = (q.cols + 127) / 128;
   if (q.block_rows == 1) {
@@ -31,12 +32,14 @@ int32_t quantize_typed(const VecopsB200QuantizeBlocks& q, int sms, VecopsError* 
     const int64_t want = (blocks + per_cta - 1) / per_cta;
     const unsigned grid = static_cast<unsigned>(want < most ? want : most);
     if (vec) f8_quantize_rows_kernel<T><<<grid, 256, 0, stream>>>(p);
+    else if (unaligned) f8_quantize_unaligned_rows_kernel<T><<<grid, 256, 0, stream>>>(p);
     else f8_quantize_strided_kernel<T><<<grid, 256, 0, stream>>>(p);
     return decode_launched("quantize_blocks", error);
   }
   const dim3 grid(static_cast<unsigned>(col_blocks), static_cast<unsigned>((q.rows + 127) / 128));
   if (grid.y > 65535u) return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "quantize_blocks: more than 65535 x 128 rows");
   if (vec) f8_quantize_tiles_kernel<T, true><<<grid, 256, 0, stream>>>(p);
+  else if (unaligned) f8_quantize_unaligned_tiles_kernel<T><<<grid, 256, 0, stream>>>(p);
   else f8_quantize_tiles_kernel<T, false><<<grid, 256, 0, stream>>>(p);
   return decode_launched("quantize_blocks", error);
 }

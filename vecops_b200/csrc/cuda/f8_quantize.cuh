@@ -124,6 +124,20 @@ __device__ __forceinline__ void f8_store_raw(uint8_t* dst, const uint4& raw, flo
   }
 }
 
+// Four elements, scaled, rounded and stored in one word (dst is on a 4-byte boundary); `left` of them are inside the row.
+__device__ __forceinline__ void f8_store4(uint8_t* dst, const float (&x)[4], float factor, int left) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * factor, x[1] * factor), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * factor, x[3] * factor), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t word = lo | hi << 16;
+  if (left >= 4) {
+    *reinterpret_cast<uint32_t*>(dst) = word;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) dst[e] = static_cast<uint8_t>(word >> (8 * e));
+  }
+}
+
 // 1 x 128 blocks of rows that allow 16-byte loads: eight threads a block, the elements held as loaded between the maximum
 // and the conversion; two blocks' loads in flight per thread.  One division a block gives both the factor (lanes 0..6) and the
 // scale (lane 7).  Instructions bound it as much as memory does: 20 an element, in a first form that converted before it
@@ -190,6 +204,58 @@ __global__ void __launch_bounds__(256) f8_quantize_rows_kernel(const F8QuantizeA
   }
 }
 
+// 1 x 128 blocks of rows that are contiguous but off 16-byte boundaries: sixteen threads a block, twice four neighbouring
+// elements each, one load an element, two blocks' loads in flight together.
+template <typename T>
+__global__ void __launch_bounds__(256) f8_quantize_unaligned_rows_kernel(const F8QuantizeArgs p) {
+  constexpr int kTogether = 2;
+  const int col_blocks = static_cast<int>((p.cols + F8Quantize::kBlock - 1) / F8Quantize::kBlock);
+  const int lane = threadIdx.x & 15;
+  const unsigned members = 0xffffu << (threadIdx.x & 16);
+  const long long step = gridDim.x * 16ll;
+  const long long step_rows = step / col_blocks;
+  const int step_cols = static_cast<int>(step - step_rows * col_blocks);
+  const long long start = blockIdx.x * 16ll + (threadIdx.x >> 4);
+  long long row = start / col_blocks;
+  int col_block = static_cast<int>(start - row * col_blocks);
+  while (row < p.rows) {
+    T raw[kTogether][2][4];
+    long long rows[kTogether];
+    int cols[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      rows[i] = row, cols[i] = col_block;
+      const T* src = static_cast<const T*>(p.src) + row * p.src_sr + col_block * F8Quantize::kBlock + lane * 4;
+      const int left = row < p.rows ? static_cast<int>(min(128ll, p.cols - col_block * static_cast<long long>(F8Quantize::kBlock))) - lane * 4 : 0;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[i][half][e] = half * 64 + e < left ? src[half * 64 + e] : T(0.f);
+      row += step_rows, col_block += step_cols;
+      if (col_block >= col_blocks) col_block -= col_blocks, ++row;
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      if (rows[i] >= p.rows) break;
+      float x[2][4], amax = 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[half][e] = f8_source(raw[i][half][e]), amax = fmaxf(amax, fabsf(x[half][e]));
+#pragma unroll
+      for (int offset = 8; offset > 0; offset >>= 1) amax = fmaxf(amax, __shfl_xor_sync(members, amax, offset));
+      amax = f8_bounded_amax(amax);
+      const float ratio = (lane == 15 ? amax : F8Quantize::kMax) / (lane == 15 ? F8Quantize::kMax : amax);
+      const float factor = __shfl_sync(members, ratio, 0, 16);
+      if (lane == 15) p.scale[rows[i] * p.scale_sr + cols[i] * p.scale_sc] = ratio;
+      uint8_t* dst = p.dst + rows[i] * p.dst_sr + cols[i] * static_cast<long long>(F8Quantize::kBlock) + lane * 4;
+      const int left = static_cast<int>(min(128ll, p.cols - cols[i] * static_cast<long long>(F8Quantize::kBlock))) - lane * 4;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) f8_store4(dst + half * 64, x[half], factor, left - half * 64);
+    }
+  }
+}
+
 // 1 x 128 blocks of any strides: sixteen threads per block, eight elements each.
 template <typename T>
 __global__ void __launch_bounds__(256) f8_quantize_strided_kernel(const F8QuantizeArgs p) {
@@ -209,6 +275,47 @@ __global__ void __launch_bounds__(256) f8_quantize_strided_kernel(const F8Quanti
     f8_store8<false>(p.dst + row * p.dst_sr, col, p.cols, x, F8Quantize::kMax / amax);
     if (lane == 0) p.scale[row * p.scale_sr + col_block * p.scale_sc] = amax / F8Quantize::kMax;
   }
+}
+
+// 128 x 128 blocks of contiguous rows off 16-byte boundaries: a row a warp at a time, four neighbouring elements a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) f8_quantize_unaligned_tiles_kernel(const F8QuantizeArgs p) {
+  constexpr int kLoads = F8Quantize::kBlock / 8;
+  __shared__ float warp_amax[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row0 = blockIdx.y * static_cast<long long>(F8Quantize::kBlock) + warp;
+  const long long col = blockIdx.x * static_cast<long long>(F8Quantize::kBlock) + lane * 4;
+  const int left = static_cast<int>(max(0ll, min(4ll, p.cols - col)));
+  T raw[kLoads][4];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const long long row = row0 + 8 * i;
+    const T* src = static_cast<const T*>(p.src) + row * p.src_sr + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) raw[i][e] = row < p.rows && e < left ? src[e] : T(0.f);
+  }
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(f8_source(raw[i][e])));
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, offset));
+  if (lane == 0) warp_amax[warp] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) amax = fmaxf(amax, warp_amax[w]);
+  amax = f8_bounded_amax(amax);
+  const float factor = F8Quantize::kMax / amax;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const long long row = row0 + 8 * i;
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = f8_source(raw[i][e]);
+    if (row < p.rows) f8_store4(p.dst + row * p.dst_sr + col, x, factor, left);
+  }
+  if (threadIdx.x == 0) p.scale[blockIdx.y * p.scale_sr + blockIdx.x * p.scale_sc] = amax / F8Quantize::kMax;
 }
 
 // 128 x 128 blocks: one CTA per block holds it, as loaded, in registers between the maximum and the conversion.

@@ -299,32 +299,34 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
       for (int slab = 0; slab < 128 / kSlabCols; ++slab) {
         if (col0 + slab * kSlabCols >= p.n || row0 >= p.m) continue;  // (uniform over the warp)
-        if (tma_store) {
-          uint32_t w[32];
+        // (TMA clips rows of C to whole 16 bytes, not to elements: a row that ends in between ends by the other way)
+        const bool by_tma = tma_store && (p.n % (16 / static_cast<int>(sizeof(OutT))) == 0 || col0 + (slab + 1) * kSlabCols <= p.n);
+        uint32_t w[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if constexpr (sizeof(OutT) == 2) {
-              const float2 f = total[slab * 32 + e];
-              w[e] = pack_out16x2<OutT>(f.x, f.y);
-            } else {
-              const float2 f = total[slab * 16 + e / 2];
-              w[e] = __float_as_uint(e & 1 ? f.y : f.x);
+        for (int e = 0; e < 32; ++e) {
+          if constexpr (sizeof(OutT) == 2) {
+            const float2 f = total[slab * 32 + e];
+            w[e] = pack_out16x2<OutT>(f.x, f.y);
+          } else {
+            const float2 f = total[slab * 16 + e / 2];
+            w[e] = __float_as_uint(e & 1 ? f.y : f.x);
+          }
+        }
+#pragma unroll 1
+        for (int part = 0; part < 32 / G::kOutRows; ++part) {
+          if (tma_store && lane == 0) tma_store_wait_read<G::kOutBuffers - 1>();  // what was in this buffer has left it
+          __syncwarp();
+          const uint32_t out_buf = out_ring + out_at * (G::kOutRows * 128);
+          if (++out_at == G::kOutBuffers) out_at = 0;
+          if (lane / G::kOutRows == part) {
+#pragma unroll
+            for (int piece = 0; piece < 8; ++piece) {
+              const uint32_t dst = out_buf + (lane % G::kOutRows) * 128 + ((piece ^ (lane & 7)) << 4);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[4 * piece]), "r"(w[4 * piece + 1]), "r"(w[4 * piece + 2]),
+                           "r"(w[4 * piece + 3]) : "memory");
             }
           }
-#pragma unroll
-          for (int part = 0; part < 32 / G::kOutRows; ++part) {
-            if (lane == 0) tma_store_wait_read<G::kOutBuffers - 1>();  // what was in this buffer has left it
-            __syncwarp();
-            const uint32_t out_buf = out_ring + out_at * (G::kOutRows * 128);
-            if (++out_at == G::kOutBuffers) out_at = 0;
-            if (lane / G::kOutRows == part) {
-#pragma unroll
-              for (int piece = 0; piece < 8; ++piece) {
-                const uint32_t dst = out_buf + (lane % G::kOutRows) * 128 + ((piece ^ (lane & 7)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[4 * piece]), "r"(w[4 * piece + 1]), "r"(w[4 * piece + 2]),
-                             "r"(w[4 * piece + 3]) : "memory");
-              }
-            }
+          if (by_tma) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -332,14 +334,30 @@ f8_tiled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
               if (row0 + part * G::kOutRows < p.m) tma_store_2d(&map_c, out_buf, col0 + slab * kSlabCols, row0 + part * G::kOutRows);
               tma_store_commit();
             }
-          }
-        } else if (row0 + lane < p.m) {
-          OutT* c = static_cast<OutT*>(p.c) + (row0 + lane) * p.c_sm;
+          } else {
+            // Rows of C that TMA cannot address - off 16-byte boundaries, or strided - leave element by element, neighbouring lanes with
+            // neighbouring columns.  (A thread storing the row it owns made 4096 x 14335 x 4096 three times as slow as 14336 columns.)
+            __syncwarp();
+            if (tma_store && lane == 0) tma_store_commit();  // (an empty one: the buffers are counted by their groups)
+            constexpr int kPer16 = 16 / static_cast<int>(sizeof(OutT));
+            const OutT* staged = reinterpret_cast<const OutT*>(smem_gen + (out_buf - smem_base));
+            const int first = row0 + part * G::kOutRows, rows = min(G::kOutRows, p.m - first);
+            const int col = col0 + slab * kSlabCols + lane;
+            OutT* c = static_cast<OutT*>(p.c) + first * p.c_sm + col * p.c_sn;
+#pragma unroll 1
+            for (int r0 = 0; r0 < rows; r0 += 4, c += 4 * p.c_sm) {
+              OutT x[4][kSlabCols / 32];  // (all on their way before the first is stored)
 #pragma unroll
-          for (int j = 0; j < kSlabCols; ++j) {
-            const int col = col0 + slab * kSlabCols + j;
-            const float2 f = total[(slab * kSlabCols + j) / 2];
-            if (col < p.n) c[col * p.c_sn] = f8_out<OutT>(j & 1 ? f.y : f.x);
+              for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < kSlabCols / 32; ++j)
+                  x[r][j] = staged[(r0 + r) * kSlabCols + (((32 * j + lane) / kPer16) ^ ((r0 + r) & 7)) * kPer16 + lane % kPer16];
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < kSlabCols / 32; ++j)
+                  if (r0 + r < rows && col + 32 * j < p.n) c[r * p.c_sm + 32 * j * p.c_sn] = x[r][j];
+            }
           }
         }
       }
