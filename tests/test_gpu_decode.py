@@ -651,6 +651,25 @@ def test_prefix_attention_ignores_query_tokens_that_do_not_exist(ops):
         assert torch.equal(ops.sdpa_shared_prefix(**outside), whole), d
 
 
+@pytest.mark.parametrize("page", [8, 16, 48, 128, 256])
+@pytest.mark.parametrize("batch,prefix", [(3, 500), (160, 500), (3, 16), (160, 16), (1, 5000), (160, 128)])
+def test_prefix_attention_whether_few_or_many_read_the_prefix(ops, batch, prefix, page):
+    # 3 sequences read it in front of their suffixes, 160 by a kernel of its own; drafted tokens, idle slots, empty suffixes, absent pages, NaN behind the keys
+    counts = [(1, 3, 0, 2)[i % 4] for i in range(batch)]
+    lengths = [(5, 3, -1, 40)[i % 4] for i in range(batch)]
+    if batch > 3:
+        lengths[0], lengths[4] = 0, 0
+    inputs = prefix_inputs(counts, lengths, prefix, 16, 8, 128, page, BF16, batch + prefix + page)
+    if prefix > 2 * page:
+        inputs["prefix_pages"][1] = -1
+    if prefix % page:
+        last = int(inputs["prefix_pages"][-1])
+        if last >= 0:
+            inputs["k_cache"][last, prefix % page:] = math.nan
+            inputs["v_cache"][last, prefix % page:] = math.nan
+    check_prefix(ops, inputs)
+
+
 # ------------------------------------------------------------------------------------------------ together, captured, on other streams
 
 def decode_step(ops, x, weights, k_cache, v_cache, tables, hq, hkv, d):

@@ -102,10 +102,18 @@ PrefixSdpaArgs prefix_args(const VecopsB200PrefixAttention& a) {
 
 // ---------------------------------------------------------------- the two-kernel form: prefix on tcgen05, suffix and merge behind it
 
+// Few sequences behind a short prefix, or one behind any: the suffix kernel reads the prefix for every item, in front of its suffix, and
+// there is no prefix kernel, if what is read again comes to no more than this.  With / without the prefix kernel, 128-dim heads
+// unless told otherwise: 12 sequences of 2 heads of 64 behind 644 keys (4 MB again) 10.0 / 8.1 us, 4 of 8 behind 512 (6 MB) 9.9 / 10.5
+// and a launch less, 183 of 1 behind 209 (19 MB) 16.0 / 12.2, one of 8 behind 16384 (none) 23.5 / 17.6; 16 of 8 behind
+// 1000 (61 MB) 15.8 / 17.3, 7 of 8 of 64 behind 4877 (60 MB) 13.2 / 18.4.
+constexpr int64_t kRereadBytes = INT64_C(32) << 20;
+
 struct PrefixPlan {
   bool fast = false;  // the two kernels can address this call; the one-warp-per-row kernel serves the rest
   int dim = 0;        // head dims a kernel is built for: 64 or 128
   int both_rows = 0, row_blocks = 0, tiles = 0, tiles_per_chunk = 0, chunks = 0, records = 0;
+  int prefix_slices = 0;  // joined: no prefix kernel, every item of the suffix kernel starts with the prefix
   int tokens_per_item = 1, group_tiles = 1, item_rows = 1, workers = 0;
   int64_t slots = 0, fragments = 0;
   uint64_t ml_at = 0, fragment_o_at = 0, fragment_ml_at = 0, sums_at = 0, total = 0;
@@ -127,7 +135,14 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
   if (!p.fast) return p;
   p.dim = a.head_dim <= 64 ? 64 : 128;
   const int64_t group = a.q_heads / a.kv_heads, rows = a.tokens * group;
-  if (a.prefix_len > 0 && a.tokens > 0 && a.pages > 0) {
+  p.tokens_per_item = static_cast<int>(group <= 16 ? 16 / group : 1);
+  p.group_tiles = static_cast<int>((group + 15) / 16);
+  p.item_rows = static_cast<int>(group >= 16 ? 16 : (a.query_starts == nullptr ? 1 : p.tokens_per_item) * group);
+  p.slots = a.query_starts == nullptr ? a.batch : a.tokens / p.tokens_per_item + a.batch + 1;
+  const int64_t columns = a.kv_heads * p.group_tiles;
+  const bool prefix = a.prefix_len > 0 && a.tokens > 0 && a.pages > 0;
+  if (prefix && p.slots * p.group_tiles - 1 <= kRereadBytes / (a.kv_heads * a.prefix_len * p.dim * 4)) p.prefix_slices = static_cast<int>((a.prefix_len + 15) / 16);
+  if (prefix && p.prefix_slices == 0) {
     p.both_rows = rows > 128 ? 1 : 0;
     p.row_blocks = static_cast<int>(p.both_rows ? (rows + 255) / 256 : 1);
     p.tiles = static_cast<int>((a.prefix_len + 127) / 128);
@@ -147,12 +162,8 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
     }
     p.records = p.both_rows ? p.chunks : 2 * p.chunks;
   }
-  p.tokens_per_item = static_cast<int>(group <= 16 ? 16 / group : 1);
-  p.group_tiles = static_cast<int>((group + 15) / 16);
-  p.item_rows = static_cast<int>(group >= 16 ? 16 : (a.query_starts == nullptr ? 1 : p.tokens_per_item) * group);
-  p.slots = a.query_starts == nullptr ? a.batch : a.tokens / p.tokens_per_item + a.batch + 1;
   // warps for every slice the table could hold, up to what the SMs hold at once (slices are counted in 32 bits)
-  const int64_t slices = (a.table_width * a.page_size + 15) / 16, columns = a.kv_heads * p.group_tiles;
+  const int64_t slices = p.prefix_slices + (a.table_width * a.page_size + 15) / 16;
   if (slices > 0 && p.slots * columns > ((INT64_C(1) << 31) - 1) / (slices + kItemWeight)) {
     p.fast = false;
     return p;
@@ -191,8 +202,8 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   static std::atomic<bool> raised[64];
   if (device.index >= 64 || !raised[device.index].load()) {
     cudaError_t status = cudaFuncSetAttribute(prefix_sdpa_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmemBytes);
-    if (status == cudaSuccess) status = cudaFuncSetAttribute(suffix_sdpa_kernel<T, kDim, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SuffixSdpa<kDim>::kSmemBytes);
-    if (status == cudaSuccess) status = cudaFuncSetAttribute(suffix_sdpa_kernel<T, kDim, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SuffixSdpa<kDim>::kSmemBytes);
+    for (auto kernel : {suffix_sdpa_kernel<T, kDim, true, false>, suffix_sdpa_kernel<T, kDim, false, false>, suffix_sdpa_kernel<T, kDim, true, true>, suffix_sdpa_kernel<T, kDim, false, true>})
+      if (status == cudaSuccess) status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SuffixSdpa<kDim>::kSmemBytes);
     if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "cudaFuncSetAttribute(prefix_sdpa): %s", cudaGetErrorString(status));
     if (device.index < 64) raised[device.index].store(true);
   }
@@ -233,7 +244,7 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   s.rows = rows;
   s.tokens_per_item = plan.tokens_per_item, s.group_tiles = plan.group_tiles, s.item_rows = plan.item_rows;
   s.slots = static_cast<int>(plan.slots), s.workers = plan.workers;
-  s.records = plan.records, s.partial_o = partial_o, s.partial_ml = partial_ml;
+  s.records = plan.records, s.prefix_slices = plan.prefix_slices, s.partial_o = partial_o, s.partial_ml = partial_ml;
   char* base = static_cast<char*>(a.workspace);
   s.fragment_o = reinterpret_cast<float*>(base + plan.fragment_o_at), s.fragment_ml = reinterpret_cast<float2*>(base + plan.fragment_ml_at);
   s.sums = reinterpret_cast<int*>(base + plan.sums_at);
@@ -241,7 +252,10 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   config.blockDim = dim3(SuffixSdpa<kDim>::kThreads);
   config.dynamicSmemBytes = SuffixSdpa<kDim>::kSmemBytes;
   config.numAttrs = 1;
-  cudaError_t status = a.page_size % 16 == 0 ? cudaLaunchKernelEx(&config, suffix_sdpa_kernel<T, kDim, true>, s) : cudaLaunchKernelEx(&config, suffix_sdpa_kernel<T, kDim, false>, s);
+  const bool whole_pages = a.page_size % 16 == 0, joined = plan.prefix_slices > 0;
+  const auto suffix = whole_pages ? (joined ? suffix_sdpa_kernel<T, kDim, true, true> : suffix_sdpa_kernel<T, kDim, true, false>)
+                                  : (joined ? suffix_sdpa_kernel<T, kDim, false, true> : suffix_sdpa_kernel<T, kDim, false, false>);
+  cudaError_t status = cudaLaunchKernelEx(&config, suffix, s);
   if (status != cudaSuccess) return set_error(error, VECOPS_STATUS_EXECUTION_ERROR, "suffix_sdpa launch: %s", cudaGetErrorString(status));
   int32_t rc = decode_launched("suffix_sdpa", error);
   if (rc != VECOPS_STATUS_OK) return rc;

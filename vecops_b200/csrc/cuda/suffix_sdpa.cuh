@@ -1,5 +1,5 @@
 // Attention over each sequence's own suffix, and the merge with what the prefix kernel left: the second and third kernels of
-// shared-prefix attention, and all of it when there is no prefix.
+// shared-prefix attention; the first and second when there is no prefix, or when few read it: every item then starts with its keys.
 //
 // An item is up to sixteen query rows of one sequence and one key/value head - the queries that read this head, of one
 // token or of a few neighbouring ones - and the keys they see, in slices of sixteen.  The work is the keys' way from
@@ -40,6 +40,7 @@ struct SuffixSdpaArgs {
   int slots;            // of items per (head, group tile), idle ones included
   int workers;          // warps of the suffix kernel
   int records;          // of the prefix kernel
+  int prefix_slices;    // without one: slices of the prefix that every item starts with (the joined form), or 0
   const float* partial_o;
   const float2* partial_ml;
   int item_rows;        // rows an item has at most
@@ -72,8 +73,8 @@ __device__ __forceinline__ int suffix_search(int batch, const Before& before) {
 }
 
 // Slices and weight of the item whose newest token is `last`.
-__device__ __forceinline__ int suffix_slices(const PrefixSdpaArgs& a, int length, int newest, int last) {
-  return length <= 0 ? 0 : (suffix_sees(a, length, newest, last) + 15) / 16;
+__device__ __forceinline__ int suffix_slices(const PrefixSdpaArgs& a, int prefix_slices, int length, int newest, int last) {
+  return length < 0 ? 0 : prefix_slices + (suffix_sees(a, length, newest, last) + 15) / 16;
 }
 __device__ __forceinline__ int suffix_weight(int slices) { return slices > 0 ? slices + kItemWeight : 0; }
 
@@ -118,14 +119,16 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) {
   return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
-// kWholePages: page_size is a multiple of sixteen, so a slice lies in one page.
-template <typename T, int kDim, bool kWholePages>
+// kWholePages: page_size is a multiple of sixteen, so a slice lies in one page.  kJoined: there is no prefix kernel, and an item's slices
+// are those of the prefix, then those of its suffix.
+template <typename T, int kDim, bool kWholePages, bool kJoined>
 __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::kCtasPerSm) suffix_sdpa_kernel(const SuffixSdpaArgs p) {
   using G = SuffixSdpa<kDim>;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t smem_base = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PrefixSdpaArgs& a = p.a;
+  const int prefix_slices = kJoined ? p.prefix_slices : 0;
   volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(smem + G::kProbOffset + G::kWarps * G::kProbBytes) + warp * G::kStages;
   if (p.records == 0) grid_dependency_wait();  // (with a prefix kernel in between, the kernels before that one are done already)
   grid_launch_dependents();
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
     const int length = a.lengths[b];
     const Tokens tokens = tokens_of(b);
     for (int first = tokens.begin; first < tokens.end; first += p.tokens_per_item)
-      sum += suffix_weight(suffix_slices(a, length, tokens.end - 1, min(tokens.end, first + p.tokens_per_item) - 1));
+      sum += suffix_weight(suffix_slices(a, prefix_slices, length, tokens.end - 1, min(tokens.end, first + p.tokens_per_item) - 1));
   }
   int before = sum;
 #pragma unroll
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
   while (position < end) {
     for (;;) {  // on to the slot that has the position
       if (first < tokens.end) {
-        slices = suffix_slices(a, length, tokens.end - 1, min(tokens.end, first + p.tokens_per_item) - 1);
+        slices = suffix_slices(a, prefix_slices, length, tokens.end - 1, min(tokens.end, first + p.tokens_per_item) - 1);
         weight = suffix_weight(slices);
         if (position < (slot_sum + weight) * columns) break;
         slot_sum += weight;
@@ -208,18 +211,21 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
     constexpr int kRowsPerStep = 32 / kPieces;  // rows a warp-wide copy covers
     const int piece = lane % kPieces, sub_row = lane / kPieces;
     // pages of the next two slices, looked up ahead: the slice's own, or - pages that end inside a slice - that of this lane's key (lanes 0..15)
+    auto in_prefix = [&](int i) { return kJoined && first_slice + i < prefix_slices; };
+    auto first_key = [&](int i) { return (in_prefix(i) ? first_slice + i : first_slice + i - prefix_slices) * G::kKeys; };  // of slice i, in its own sequence
     int page_slot = 0, page_offset = 0;  // where the slice to be looked up next starts
-    if constexpr (kWholePages) page_slot = first_slice * G::kKeys / a.page_size, page_offset = first_slice * G::kKeys - page_slot * a.page_size;
+    if constexpr (kWholePages) page_slot = first_key(0) / a.page_size, page_offset = first_key(0) - page_slot * a.page_size;
     int look = 0;
     auto page_of_next = [&] {
       int page = -1;
       if constexpr (kWholePages) {
-        if (look < mine && page_slot < a.table_width) page = __ldg(pages + page_slot);
+        if (kJoined && first_slice + look == prefix_slices) page_slot = page_offset = 0;
+        if (look < mine && (in_prefix(look) || page_slot < a.table_width)) page = __ldg((in_prefix(look) ? a.prefix_pages : pages) + page_slot);
         page_offset += G::kKeys;
         if (page_offset >= a.page_size) page_offset = 0, ++page_slot;
       } else {
-        const int key = (first_slice + look) * G::kKeys + (lane & 15);
-        if (look < mine && key < some_see) page = __ldg(pages + key / a.page_size);
+        const int key = first_key(look) + (lane & 15);
+        if (look < mine && key < (in_prefix(look) ? a.prefix_len : some_see)) page = __ldg((in_prefix(look) ? a.prefix_pages : pages) + key / a.page_size);
       }
       ++look;
       return page;
@@ -236,7 +242,8 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
         uint32_t mask;
         long long k_at = 0, v_at = 0;
         if constexpr (kWholePages) {
-          const int keys = min(G::kKeys, some_see - (first_slice + i) * G::kKeys);
+          const int keys = min(G::kKeys, (in_prefix(i) ? a.prefix_len : some_see) - first_key(i));
+          if (kJoined && first_slice + i == prefix_slices) offset_next = 0;
           mask = there ? 0xffffu >> (16 - keys) : 0u;
           if (there) {
             k_at = page * a.k_sp + (offset_next + sub_row) * a.k_ss, v_at = page * a.v_sp + (offset_next + sub_row) * a.v_ss;
@@ -245,7 +252,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
           if (offset_next >= a.page_size) offset_next = 0;
         } else {
           mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
-          const long long offset = ((first_slice + i) * G::kKeys + (lane & 15)) % a.page_size;
+          const long long offset = (first_key(i) + (lane & 15)) % a.page_size;
           if (there) k_at = page * a.k_sp + offset * a.k_ss, v_at = page * a.v_sp + offset * a.v_ss;
         }
         if (lane == 0) present[stage] = mask;
@@ -304,7 +311,8 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
       }
       cp_async_wait<G::kStages - 1>();
       __syncwarp();
-      const int stage = i % G::kStages, key0 = (first_slice + i) * G::kKeys;
+      const int stage = i % G::kStages, key0 = first_key(i);
+      const bool of_prefix = in_prefix(i);  // (every row sees it)
       const uint32_t k_tile = ring + stage * 2 * G::kTileBytes, v_tile = k_tile + G::kTileBytes;
       float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -322,7 +330,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = nt * 8 + (lane & 3) * 2 + (e & 1);
-          const bool keep = key0 + key < sees[e >> 1] && (mask >> key & 1u) != 0;
+          const bool keep = (of_prefix || key0 + key < sees[e >> 1]) && (mask >> key & 1u) != 0;
           s[nt][e] = keep ? s[nt][e] * scale : -INFINITY;
           top[e >> 1] = fmaxf(top[e >> 1], s[nt][e]);
         }
@@ -354,7 +362,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
           s[nt][e] = exp2_approx(s[nt][e] - base);
           l[e >> 1] += s[nt][e];
         }
-      if (key0 + G::kKeys > all_see && all_see < some_see) {
+      if (!of_prefix && key0 + G::kKeys > all_see && all_see < some_see) {
         // keys that not every row sees: added here, one by one, where a row that does not see a key does not touch its value
         __syncwarp();
 #pragma unroll
@@ -444,11 +452,11 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
   owned = owned && length >= 0;
   int fragments = 0;
   size_t first_fragment = 0;  // its row in the fragments
-  if (owned && length > 0) {
+  if (owned) {
     const int tile = (t - start) / p.tokens_per_item, first = start + tile * p.tokens_per_item;
     const int slot = a.query_starts != nullptr ? start / p.tokens_per_item + sequence + tile : sequence;
     const int last = min(newest, first + p.tokens_per_item - 1);
-    const int slices = suffix_slices(a, length, newest, last), weight = suffix_weight(slices);
+    const int slices = suffix_slices(a, p.prefix_slices, length, newest, last), weight = suffix_weight(slices);
     if (slices > 0) {
       const int columns = a.kv_heads * p.group_tiles, column = kv * p.group_tiles + in_group / 16;
       const int all = __ldcg(p.sums + p.slots) * columns, from = __ldcg(p.sums + slot) * columns + column * weight, workers = min(p.workers, all);
