@@ -437,10 +437,9 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
   const bool there = index < static_cast<long long>(a.tokens) * a.q_heads;
   const int t = there ? static_cast<int>(index / a.q_heads) : 0, head = there ? static_cast<int>(index - static_cast<long long>(t) * a.q_heads) : 0;
   const int kv = head / a.group, in_group = head - kv * a.group;
-  grid_dependency_wait();
-  grid_launch_dependents();
 
-  // the row's sequence, item and fragments
+  // the row's sequence (the suffix kernel lets this one start only when the kernels before the attention are done: what they
+  // wrote is read without waiting for it)
   int sequence = t, start = t, newest = t;
   bool owned = there;
   if (a.query_starts != nullptr) {
@@ -450,6 +449,9 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
   }
   const int length = owned ? a.lengths[sequence] : -1;
   owned = owned && length >= 0;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  // its item and fragments
   int fragments = 0;
   size_t first_fragment = 0;  // its row in the fragments
   if (owned) {
