@@ -14,6 +14,10 @@
 // sums rows m = r (mod S) of all slices, in slice order, so results do not depend on timing.  The store is a loop over
 // shared memory, not code unrolled over the registers: instructions that run once are fetched at about 100 cycles a
 // line, and 64 rows of unrolled stores took 5 us.
+//
+// Measured: 1 x 14336 x 4096 (58.7 MB of weights) 12.5 us in a graph, 4.7 TB/s: the stream itself runs at 7.3 TB/s, above what a
+// copy reaches, and starting, the slices' meeting and the store are the other 3.7 us.  61 x 4100 x 4176: 8.2 us.  What is in
+// flight decides: with the rings half as deep the two took 13.8 and 15.6 us.
 #pragma once
 
 #include "f8_generic.cuh"

@@ -19,8 +19,14 @@
 //               accumulators); what it waits for is kept to one barrier per step and one per group, as a wait costs it
 //               some 150 cycles even when there is nothing to wait for
 //   warps 4-19  two softmax groups; they also bring Q to shared memory
-// A work item is (row block, head, chunk of key tiles); each group leaves (O, m, l) of its rows in scratch, and the suffix
-// kernel, launched behind, merges them.  Every wait is bounded.
+// A work item is (row block, head, chunk of key tiles); each group leaves (O, m, l) of its rows in scratch, and the merge
+// kernel joins them.  Every wait is bounded.
+//
+// Measured: 256 sequences of 32 query heads behind 32768 keys of 8 heads of 128 (137 GFLOP): 138 us with the merge, 990 TFLOP/s,
+// 0.59 of the measured bf16 rate, at 1.64 GHz under the power limit; the tensor pipe is busy 57 % of the time, the
+// special-function pipe 43 %, and a step of both groups takes some 3500 cycles for 2048 of MMAs - each group's chain of
+// products and softmax, of which only half lies under the other group's.  Few rows are bound by what a call begins and ends
+// with: some 4500 cycles to the first scores, 1500 to 3500 for the record.
 #pragma once
 
 #include <math.h>

@@ -1,7 +1,8 @@
 // Shared-prefix attention, one warp per query row: for head dims, strides and alignments the tensor-core kernels cannot
 // address.  The keys are walked one by one with a running maximum m and sum l,
 //     m' = max(m, s)   l = l e^(m - m') + e^(s - m')   O = O e^(m - m') + e^(s - m') v      out = O / l
-// in fp32; a lane holds head_dim / 32 of q and O.
+// in fp32; a lane holds head_dim / 32 of q and O.  Bound by the latency of a key after the other: 64 sequences behind 8192 keys of
+// 8 heads of 128 take 16.5 ms (the tensor-core kernels: 53 us).
 #pragma once
 
 #include <math.h>
