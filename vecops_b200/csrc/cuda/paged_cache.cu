@@ -114,7 +114,7 @@ struct PrefixPlan {
   int dim = 0;        // head dims a kernel is built for: 64 or 128
   int both_rows = 0, row_blocks = 0, tiles = 0, tiles_per_chunk = 0, chunks = 0, records = 0;
   int prefix_slices = 0;  // joined: no prefix kernel, every item of the suffix kernel starts with the prefix
-  int tokens_per_item = 1, group_tiles = 1, item_rows = 1, workers = 0;
+  int tokens_per_item = 1, group_tiles = 1, item_rows = 1, workers = 0, beside = 0, beside_most = 0;
   int64_t slots = 0, fragments = 0;
   uint64_t ml_at = 0, fragment_o_at = 0, fragment_ml_at = 0, sums_at = 0, total = 0;
 };
@@ -173,6 +173,16 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
   wanted = slices == 0 || wanted >= most ? (slices == 0 ? 1 : most) : (wanted * slices < most ? wanted * slices : most);
   p.workers = static_cast<int>((wanted + 3) / 4 * 4);
   p.fragments = p.workers + p.slots * columns;
+  if (p.records > 0) {
+    // Suffixes that are done before the prefix kernel is, on the SMs that it leaves: a position (a slice of 16 keys) takes a warp up to
+    // 1 us there, the prefix kernel 2 us a key tile and four tiles more.  On all SMs / on those: 64 sequences of 8 heads behind
+    // 512 keys 18.6 / 14.6 us, 64 of 4 behind 1066 14.7 / 11.2; and 256 of 8 behind 32768, which take longer, 183 / 277.
+    const int64_t free_sms = sms - a.kv_heads * p.row_blocks * p.chunks;
+    const int64_t beside = free_sms <= 0 ? 0 : free_sms * SuffixSdpa<64>::kCtasPerSm * SuffixSdpa<64>::kWarps;
+    p.beside = static_cast<int>(beside < p.workers ? beside : p.workers);
+    const int64_t positions = 2 * (static_cast<int64_t>(p.tiles_per_chunk) + 4);
+    p.beside_most = p.beside * static_cast<int>(positions < (1 << 16) ? positions : (1 << 16));
+  }
 
   auto place = [&](uint64_t bytes) {
     const uint64_t at = p.total;
@@ -243,7 +253,7 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
   s.a = args;
   s.rows = rows;
   s.tokens_per_item = plan.tokens_per_item, s.group_tiles = plan.group_tiles, s.item_rows = plan.item_rows;
-  s.slots = static_cast<int>(plan.slots), s.workers = plan.workers;
+  s.slots = static_cast<int>(plan.slots), s.workers = plan.workers, s.beside = plan.beside, s.beside_most = plan.beside_most;
   s.records = plan.records, s.prefix_slices = plan.prefix_slices, s.partial_o = partial_o, s.partial_ml = partial_ml;
   char* base = static_cast<char*>(a.workspace);
   s.fragment_o = reinterpret_cast<float*>(base + plan.fragment_o_at), s.fragment_ml = reinterpret_cast<float2*>(base + plan.fragment_ml_at);

@@ -43,6 +43,8 @@ struct SuffixSdpaArgs {
   int group_tiles;      // items a token is cut into when its group has more than sixteen heads
   int slots;            // of items per (head, group tile), idle ones included
   int workers;          // warps of the suffix kernel
+  int beside;           // ... that there is room for beside the prefix kernel's CTAs
+  int beside_most;      // what may be dealt to them
   int records;          // of the prefix kernel
   int prefix_slices;    // without one: slices of the prefix that every item starts with (the joined form), or 0
   const float* partial_o;
@@ -56,6 +58,12 @@ struct SuffixSdpaArgs {
 // Without query_starts slot b is sequence b's one token; with them sequence b's items are the slots from
 // query_starts[b] / tokens_per_item + b on: apart from each other, and found without a sum.
 constexpr int kItemWeight = 2;  // slices' worth of time that an item's lookups, queries and fragment take (measured: 2.5 us of 1 to 2 us each)
+
+// Warps that `all` is dealt to: two positions at least to each - a slice's fragment costs the merge as much as the slice - and, if
+// they would be done before the prefix kernel is, no more than there is room for beside it: CTAs that do not fit start when it ends.
+__device__ __forceinline__ int suffix_workers(int workers, int beside, int beside_most, int all) {
+  return min(all <= beside_most ? beside : workers, (all + 1) / 2);
+}
 
 // Suffix keys that token t sees of a sequence whose newest token is `newest`: of those the table has room for (fewer than 2^31).
 __device__ __forceinline__ int suffix_sees(const PrefixSdpaArgs& a, int length, int newest, int t) {
@@ -166,7 +174,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
   const int all = total * columns;                 // (the host has made sure that it fits)
   const int worker = static_cast<int>(blockIdx.x) * G::kWarps + warp;
   if (worker == 0 && lane == 0) p.sums[p.slots] = total;
-  const int workers = min(p.workers, all);  // (no warp is dealt nothing while another has something)
+  const int workers = suffix_workers(p.workers, p.beside, p.beside_most, all);  // (no warp is dealt nothing while another has something)
   int position = worker < workers ? static_cast<int>(static_cast<long long>(all) * worker / workers) : 0;
   const int end = worker < workers ? static_cast<int>(static_cast<long long>(all) * (worker + 1) / workers) : 0;
   // the run of sequences that the first position lies in, to be walked from its first
@@ -428,7 +436,8 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
       }
     }
   }
-  grid_dependency_wait();  // this kernel is done when the prefix kernel is, too: the merge waits for this one alone
+  // this kernel is done when the prefix kernel is, too: the merge waits for this one alone.  One CTA sees to that; the others make room
+  if (blockIdx.x == 0) grid_dependency_wait();
 }
 
 // The merge: kRowWarps warps per query row, each with its share of the row's partial results.
@@ -465,7 +474,8 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
     const int slices = suffix_slices(a, p.prefix_slices, length, newest, last), weight = suffix_weight(slices);
     if (slices > 0) {
       const int columns = a.kv_heads * p.group_tiles, column = kv * p.group_tiles + in_group / 16;
-      const int all = __ldcg(p.sums + p.slots) * columns, from = __ldcg(p.sums + slot) * columns + column * weight, workers = min(p.workers, all);
+      const int all = __ldcg(p.sums + p.slots) * columns, from = __ldcg(p.sums + slot) * columns + column * weight;
+      const int workers = suffix_workers(p.workers, p.beside, p.beside_most, all);
       auto worker_of = [&](int at) { return static_cast<int>(((at + 1ll) * workers - 1) / all); };  // whose [all w / workers, all (w + 1) / workers) has it
       const int first_worker = worker_of(from + kItemWeight);  // (the item's extra weight lies before its slices)
       fragments = worker_of(from + weight - 1) - first_worker + 1;
