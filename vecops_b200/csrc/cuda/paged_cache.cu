@@ -142,46 +142,70 @@ PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
   const int64_t columns = a.kv_heads * p.group_tiles;
   const bool prefix = a.prefix_len > 0 && a.tokens > 0 && a.pages > 0;
   if (prefix && p.slots * p.group_tiles - 1 <= kRereadBytes / (a.kv_heads * a.prefix_len * p.dim * 4)) p.prefix_slices = static_cast<int>((a.prefix_len + 15) / 16);
-  if (prefix && p.prefix_slices == 0) {
-    p.both_rows = rows > 128 ? 1 : 0;
-    p.row_blocks = static_cast<int>(p.both_rows ? (rows + 255) / 256 : 1);
-    p.tiles = static_cast<int>((a.prefix_len + 127) / 128);
-    // Cut the prefix so that the waves of work items are full.  In units of a key tile's time (2 us with two row blocks): an item
-    // costs its tiles and about four more - Q, the first loads, the record it leaves - and a record of 10000 rows of 128 dims
-    // is a tile's worth of writing and merging.
-    const int64_t base = a.kv_heads * p.row_blocks;
-    const double record_cost = static_cast<double>(a.kv_heads) * rows * p.dim / 1.28e6;
-    double best = 0;
-    for (int per_chunk = p.tiles, used = 1; used <= 128;) {
-      const int64_t waves = (base * used + sms - 1) / sms;
-      const double cost = static_cast<double>(waves) * (per_chunk + 4) + record_cost * used;
-      if (best == 0 || cost < best) best = cost, p.tiles_per_chunk = per_chunk, p.chunks = used;
-      if (per_chunk == 1) break;
-      used = (p.tiles + per_chunk - 2) / (per_chunk - 1);  // the fewest chunks that are shorter (each length once: the rest cut alike)
-      per_chunk = (p.tiles + used - 1) / used;
-    }
-    p.records = p.both_rows ? p.chunks : 2 * p.chunks;
-  }
   // warps for every slice the table could hold, up to what the SMs hold at once (slices are counted in 32 bits)
-  const int64_t slices = p.prefix_slices + (a.table_width * a.page_size + 15) / 16;
+  const int64_t table_slices = (a.table_width * a.page_size + 15) / 16, slices = p.prefix_slices + table_slices;
   if (slices > 0 && p.slots * columns > ((INT64_C(1) << 31) - 1) / (slices + kItemWeight)) {
     p.fast = false;
     return p;
   }
-  const int64_t most = static_cast<int64_t>(sms) * SuffixSdpa<64>::kCtasPerSm * SuffixSdpa<64>::kWarps;
+  constexpr int64_t kSmWarps = SuffixSdpa<64>::kCtasPerSm * SuffixSdpa<64>::kWarps;
+  const int64_t most = sms * kSmWarps;
   int64_t wanted = p.slots * columns;
   wanted = slices == 0 || wanted >= most ? (slices == 0 ? 1 : most) : (wanted * slices < most ? wanted * slices : most);
   p.workers = static_cast<int>((wanted + 3) / 4 * 4);
   p.fragments = p.workers + p.slots * columns;
-  if (p.records > 0) {
-    // Suffixes that are done before the prefix kernel is, on the SMs that it leaves: a position (a slice of 16 keys) takes a warp up to
-    // 1 us there, the prefix kernel 2 us a key tile and four tiles more.  On all SMs / on those: 64 sequences of 8 heads behind
-    // 512 keys 18.6 / 14.6 us, 64 of 4 behind 1066 14.7 / 11.2; and 256 of 8 behind 32768, which take longer, 183 / 277.
-    const int64_t free_sms = sms - a.kv_heads * p.row_blocks * p.chunks;
-    const int64_t beside = free_sms <= 0 ? 0 : free_sms * SuffixSdpa<64>::kCtasPerSm * SuffixSdpa<64>::kWarps;
-    p.beside = static_cast<int>(beside < p.workers ? beside : p.workers);
-    const int64_t positions = 2 * (static_cast<int64_t>(p.tiles_per_chunk) + 4);
-    p.beside_most = p.beside * static_cast<int>(positions < (1 << 16) ? positions : (1 << 16));
+  if (prefix && p.prefix_slices == 0) {
+    p.both_rows = rows > 128 ? 1 : 0;
+    p.row_blocks = static_cast<int>(p.both_rows ? (rows + 255) / 256 : 1);
+    p.tiles = static_cast<int>((a.prefix_len + 127) / 128);
+    // How the prefix is cut decides how many SMs it takes, and for how long; the suffixes go on the others meanwhile, or behind it.
+    // In us, as measured: an item of the prefix kernel takes 2 for a key tile and for five more - Q, the first loads, the record it
+    // leaves; a record of 10000 rows of 128 dims 2 to write and merge; the suffix kernel 5 to start, a warp of it 1.4 (64 dims: 1)
+    // a position - a slice of 16 keys, or a part of an item's start - and all of it what the memory takes; of what is left to
+    // it behind the prefix kernel, the free SMs have done one and a half times their share.  The lengths are on the device: taken to be
+    // half of the table's.  Every SM for the prefix / cut as this finds best: 64 sequences of 8 heads of 128 behind 8192 keys,
+    // up to 1024 of their own, 52.4 / 40.4 us; 128 behind 4096, 2048, 112 / 107; 192 behind 16384, 512, 98 / 92; 100 of one to
+    // three tokens behind 3000, 200, 31.7 / 28.3; 256 behind 32768, 512, 182 / 182; and where it errs, a table for 8192 keys with
+    // 100 in it, 29.3 / 34.9.
+    const int64_t base = a.kv_heads * p.row_blocks;
+    const double record_us = static_cast<double>(a.kv_heads) * rows * p.dim / 6.4e5;
+    const double position_us = 0.5 + 0.9 * p.dim / 128, start_us = 5;
+    const int64_t items = a.query_starts == nullptr || a.tokens / p.tokens_per_item < a.batch ? a.batch : a.tokens / p.tokens_per_item;
+    const double positions = table_slices == 0 ? 0 : static_cast<double>(items) * columns * (table_slices * 0.5 + (a.query_starts == nullptr ? 1 : 2) * kItemWeight);
+    auto suffix_us = [&](double warps) {
+      const double by_warps = positions / warps * position_us, by_memory = positions * 64 * p.dim / 5.5e6;
+      return start_us + (by_warps > by_memory ? by_warps : by_memory);
+    };
+    // each length of a chunk once, from the longest on: the fewest chunks that are shorter (the rest cut alike)
+    auto each_cut = [&](auto&& cut) {
+      for (int per_chunk = p.tiles, used = 1; used <= 128;) {
+        const int64_t waves = (base * used + sms - 1) / sms;
+        cut(per_chunk, used, 2.0 * waves * (per_chunk + 5));
+        if (per_chunk == 1) break;
+        used = (p.tiles + per_chunk - 2) / (per_chunk - 1);
+        per_chunk = (p.tiles + used - 1) / used;
+      }
+    };
+    double shortest = 1e30, best = 1e30;
+    each_cut([&](int, int, double prefix_us) { shortest = prefix_us < shortest ? prefix_us : shortest; });
+    each_cut([&](int per_chunk, int used, double prefix_us) {
+      if (prefix_us > 1.8 * shortest) return;  // (not at any price for the prefix: a table may be far wider than its lengths)
+      const int64_t free_sms = base * used < sms ? sms - base * used : 0;
+      const int64_t beside = free_sms * kSmWarps < p.workers ? free_sms * kSmWarps : p.workers;
+      const double all_us = suffix_us(p.workers), meanwhile = 1.5 * prefix_us * free_sms / sms;
+      const double after = prefix_us + (all_us > meanwhile ? all_us - meanwhile : 0), along = beside == 0 ? after : suffix_us(static_cast<double>(beside));
+      const double cost = record_us * used + (along < prefix_us ? prefix_us : along < after ? along : after);
+      if (cost < best) {
+        best = cost, p.tiles_per_chunk = per_chunk, p.chunks = used;
+        // Beside the prefix kernel if that ends sooner than all warps behind it, which is decided where the lengths are; a third in its
+        // favour, as CTAs that there is no room for start late.  (On all SMs / beside it: 64 sequences of 8 heads behind 512 keys
+        // 18.6 / 14.6 us, 64 of 4 behind 1066 14.7 / 11.2.)
+        p.beside = static_cast<int>(beside);
+        const double limit = beside == p.workers ? 2147483647.0 : 1.33 * prefix_us / position_us * beside * p.workers / (p.workers - beside);
+        p.beside_most = limit < 2147483647.0 ? static_cast<int>(limit) : 2147483647;
+      }
+    });
+    p.records = p.both_rows ? p.chunks : 2 * p.chunks;
   }
 
   auto place = [&](uint64_t bytes) {
