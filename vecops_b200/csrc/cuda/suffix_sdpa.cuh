@@ -4,9 +4,9 @@
 // An item is up to sixteen query rows of one sequence and one key/value head - the queries that read this head, of one
 // token or of a few neighbouring ones - and the keys they see, in slices of sixteen.  The work is the keys' way from
 // memory: every key and value is used by at most sixteen rows.  So all slices of all items, in order, are dealt out evenly to
-// the warps of the grid whatever the lengths are - an item counts as kItemWeight slices more, for what starting on it costs; a warp keeps the next slice in flight by cp.async while it multiplies
-// one with mma.sync m16n8k16, whose sixteen rows are the item's (tcgen05's 128 would be nearly empty).  Warps share
-// nothing and meet at no barrier.  Each runs m' = max(m, s), l, O over its part of an item and leaves them as a fragment;
+// the warps of the grid whatever the lengths are - an item counts as kItemWeight slices more, for what starting on it costs; a
+// warp keeps the next slice in flight by cp.async while it multiplies one with mma.sync m16n8k16, whose sixteen rows are the
+// item's (tcgen05's 128 would be nearly empty).  Warps share nothing and meet at no barrier.  Each runs m' = max(m, s), l, O over its part of an item and leaves them as a fragment;
 // sdpa_merge_rows_kernel, launched behind, joins a row's fragments and its prefix records,
 //     M = max m_c      out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c           (m in units of log2(e))
 // in an order that does not depend on timing.  Keys that some of an item's rows see and others do not - at most fifteen, the
@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
     if (lane == 0) p.sums[slot] = slot_sum;
     const int in_slot = position - slot_sum * columns;
     const int column = in_slot / weight, in_item = in_slot - column * weight;
+    if (column < 0 || column >= columns) break;  // (query_starts that decrease: the sums may have wrapped)
     const int stop = min(weight, in_item + end - position);
     position += stop - in_item;
     const int first_slice = max(0, in_item - kItemWeight), mine = max(0, stop - kItemWeight) - first_slice;
@@ -477,8 +478,9 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
       const int all = __ldcg(p.sums + p.slots) * columns, from = __ldcg(p.sums + slot) * columns + column * weight;
       const int workers = suffix_workers(p.workers, p.beside, p.beside_most, all);
       auto worker_of = [&](int at) { return static_cast<int>(((at + 1ll) * workers - 1) / all); };  // whose [all w / workers, all (w + 1) / workers) has it
-      const int first_worker = worker_of(from + kItemWeight);  // (the item's extra weight lies before its slices)
-      fragments = worker_of(from + weight - 1) - first_worker + 1;
+      // (kept within the fragments whatever the sums are, should query_starts decrease)
+      const int first_worker = workers <= 0 ? 0 : min(max(worker_of(from + kItemWeight), 0), workers - 1);  // (the item's extra weight lies before its slices)
+      fragments = workers <= 0 ? 0 : min(worker_of(from + weight - 1), workers - 1) - first_worker + 1;
       const int heads = min(16, a.group - in_group / 16 * 16);
       first_fragment = (static_cast<size_t>(first_worker) + static_cast<size_t>(slot) * columns + column) * p.item_rows + (t - first) * heads + in_group % 16;
     }
