@@ -42,11 +42,19 @@ struct PrefixTc {
   static constexpr int kAtoms = kDim / 64;               // 64 head dims (128 bytes) per swizzle atom
   static constexpr int kAtomBytes = 128 * 128;
   static constexpr int kTileBytes = kAtoms * kAtomBytes;  // Q, K or V: 128 rows
-  // what is left beside Q: steps of a V and a K tile.  One row block needs half the Q and has room for more of them.
+  static constexpr int kFirstSoftmaxWarp = 4, kGroupWarps = 8;
+  // Q's place, which O leaves through at the end: 2 KB a softmax warp.  The ring begins behind all of it, as one group's O leaves while
+  // the last V tile of the other is still to be multiplied.
+  static constexpr int kStageBytes = 2048;
+  __host__ __device__ static constexpr int q_bytes(bool both_rows) {
+    const int q = (both_rows ? 2 : 1) * kTileBytes, staged = 2 * kGroupWarps * kStageBytes;
+    return q > staged ? q : staged;
+  }
+  // what is left beside Q: steps of a V and a K tile.  One row block needs less for Q and has room for more of them.
   static constexpr int kSpace = 224 * 1024;
   static constexpr int kMostSteps = 6;
   __host__ __device__ static constexpr int steps(bool both_rows) {
-    const int fit = (kSpace - (both_rows ? 2 : 1) * kTileBytes) / (2 * kTileBytes);
+    const int fit = (kSpace - q_bytes(both_rows)) / (2 * kTileBytes);
     return fit < kMostSteps ? fit : kMostSteps;
   }
   static constexpr int kMaskOffset = kSpace;
@@ -57,7 +65,6 @@ struct PrefixTc {
   static constexpr int kBarriers = 2 * kMostSteps + 5;
   static constexpr int kAlign = 256;                     // of dynamic shared memory; the tiles' swizzle wants 1024
   static constexpr int kSmemBytes = kBarrierOffset + kBarriers * 8 + 8 + 1024 - kAlign;
-  static constexpr int kFirstSoftmaxWarp = 4, kGroupWarps = 8;
   static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + 2 * kGroupWarps);
   static constexpr int kPolynomialPairs = 4;             // of 16 pairs of exponentials, those computed beside the special-function units
   static constexpr int kTmemColumns = 512;               // group g: scores (and probabilities over them) at 256 g, O at 256 g + 128
@@ -154,7 +161,7 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const int row0 = row_block * (p.both_rows ? 2 * G::kRows : G::kRows);
   // K runs `lead` tiles ahead of V: steps [0, lead) bring a K tile each, step lead + t brings V tile t and K tile t + lead
   const int lead = min(p.both_rows ? 1 : 2, n), steps = G::steps(p.both_rows != 0);
-  const uint32_t ring = smem_base + (p.both_rows ? 2 : 1) * G::kTileBytes;  // Q lies before it
+  const uint32_t ring = smem_base + G::q_bytes(p.both_rows != 0);  // Q lies before it
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kMostSteps; ++s) {
@@ -443,9 +450,9 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const size_t at = (static_cast<size_t>(record) * p.a.kv_heads + kv) * p.rows + row;
     if (turn > 0) wait_scores();  // the last product is in O
     if (ok && turn > 0) {
-      // through shared memory - Q's place: every product of scores is done - so that whole 64-byte pieces of a row leave
-      // together (a thread storing its own row, 16 bytes at a time, took 6 us)
-      const uint32_t stage = smem_base + (warp - G::kFirstSoftmaxWarp) * 2048;
+      // through shared memory - Q's place: every product of scores is done, the other group's last one with V may not be - so that
+      // whole 64-byte pieces of a row leave together (a thread storing its own row, 16 bytes at a time, took 6 us)
+      const uint32_t stage = smem_base + (warp - G::kFirstSoftmaxWarp) * G::kStageBytes;
       const int first_row = row - lane;
 #pragma unroll 1
       for (int col = 0; col < kDim / 2; col += 16) {
