@@ -145,7 +145,8 @@ VECOPS_B200_EXPORT int32_t vecops_b200_cache_append(const VecopsB200CacheAppend*
  * Prefix key j lies in page prefix_pages[j / page_size], suffix key j of sequence b in page page_table[b][j / page_size].
  * Keys of a page number outside [0, pages) count as absent, as do suffix keys past the table's width.  A query that sees
  * no key, a token of no sequence and the tokens of a sequence with a negative length (padding of a captured batch) get
- * zeros.  What lies in the cache behind the last key is never used, NaN included.  lengths, query_starts and both tables
+ * zeros.  A NaN in a query or in a key that it sees gives NaN, and so do scores that are +inf or all -inf (0 / 0 by the formula).
+ * What lies in the cache behind the last key is never used, NaN included.  lengths, query_starts and both tables
  * are read on the device, so a captured call follows their later contents; prefix_len is fixed at the call. */
 typedef struct VecopsB200PrefixAttention {
   uint32_t struct_size;

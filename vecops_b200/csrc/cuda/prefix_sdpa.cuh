@@ -79,7 +79,7 @@ struct PrefixTcArgs {
   int both_rows;       // 1: the groups hold two blocks of 128 rows; 0: one block, the groups take the key tiles in turn
   int box_keys;        // keys per TMA box: min(page_size, 128)
   float* partial_o;    // [record][kv head][row][kDim]
-  float2* partial_ml;  // [record][kv head][row] (m, l)
+  float2* partial_ml;  // [record][kv head][row] (m, l); (-inf, 0) for no key, (-inf, > 0) for keys whose scores are all -inf
   uint32_t* status;
 };
 
@@ -346,8 +346,8 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const float scale = signed_scale == 0.f ? 1.f : fabsf(signed_scale);
     const unsigned long long scale2 = f2_same(scale);
     const int box_shift = 31 - __clz(p.box_keys);
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
+    float m = -INFINITY, l = 0.f;  // m is never NaN: a NaN score shows in l
+    bool ok = true, keyed = false;  // keyed: a page of the group's tiles is in the cache
     int turn = 0;
     auto wait_scores = [&] {
       if (ok && !__all_sync(0xffffffffu, mbar_wait(s_bar + 8 * g, static_cast<uint32_t>(turn) & 1u, abort_flag))) {
@@ -363,6 +363,7 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       // columns already read.  (Held in registers between the two they spilled.)
       const int last = p.a.prefix_len - (first_tile + tile) * G::kKeys - half * 64;
       const uint32_t gone = absent[tile % G::kMaskSlots];
+      keyed = keyed || __popc(gone) * p.box_keys < min(G::kKeys, last + half * 64);
       auto load_scores = [&](int col, float (&t)[32]) {
         tmem_load_32x32(my_scores + col, reinterpret_cast<uint32_t(&)[32]>(t));
         tmem_load_wait();
@@ -479,6 +480,7 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     if (half == 1) exchange[128] = l;
     meet();
     if (half == 0) l += exchange[128];
+    if (m == -INFINITY && keyed) l += 1.f;  // scores of -inf alone are keys all the same (or NaN, which l keeps)
     if (half == 0 && row < p.rows) __stcg(p.partial_ml + at, make_float2(turn > 0 && ok ? m : -INFINITY, turn > 0 && ok ? l : 0.f));
   }
 

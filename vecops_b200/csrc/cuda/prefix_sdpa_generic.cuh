@@ -92,8 +92,8 @@ __global__ void __launch_bounds__(256) prefix_sdpa_generic_kernel(const PrefixSd
     for (int offset_lane = 16; offset_lane > 0; offset_lane >>= 1) s += __shfl_xor_sync(0xffffffffu, s, offset_lane);
     s *= p.scale;
     const float m_new = fmaxf(m, s);
-    // a maximum of -inf (every score so far -inf): nothing has any weight yet
-    const float keep = m_new == -INFINITY ? 1.f : __expf(m - m_new), w = m_new == -INFINITY ? 0.f : __expf(s - m_new);
+    // while every score is -inf (or NaN, which fmaxf drops and w keeps) each key counts once: l tells that there was one
+    const float keep = m_new == -INFINITY ? 1.f : __expf(m - m_new), w = m_new != -INFINITY ? __expf(s - m_new) : s == -INFINITY ? 1.f : s;
     l = fmaf(l, keep, w);
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
@@ -102,11 +102,11 @@ __global__ void __launch_bounds__(256) prefix_sdpa_generic_kernel(const PrefixSd
     }
     m = m_new;
   }
-  const float reciprocal = keys > 0 && l != 0.f ? 1.f / l : 0.f;
+  const float reciprocal = l == 0.f ? 0.f : m == -INFINITY ? NAN : 1.f / l;  // no key: zeros; only keys whose score is -inf: 0 / 0
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
     const int d = lane + 32 * i;
-    if (d < p.head_dim) out[d] = append_down<T>(l != 0.f ? o[i] * reciprocal : 0.f);
+    if (d < p.head_dim) out[d] = append_down<T>(o[i] * reciprocal);
   }
 }
 

@@ -297,7 +297,8 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
     for (int nt = 0; nt < kDim / 8; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m is never NaN: a NaN score shows in l
+    uint32_t keyed[2] = {0u, 0u};                             // not zero: the row has seen a key
 
     for (int i = 1 - G::kStages; i < mine; ++i) {
       issue(i + G::kStages - 1);
@@ -337,14 +338,19 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
         mma_16816<T>(s[1], q[ks], b[2], b[3]);
       }
       const uint32_t mask = present[stage];
+      uint32_t visible[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        visible[h] = of_prefix ? mask : mask & ((1u << max(0, min(G::kKeys, sees[h] - key0))) - 1u);
+        keyed[h] |= visible[h];
+      }
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = nt * 8 + (lane & 3) * 2 + (e & 1);
-          const bool keep = (of_prefix || key0 + key < sees[e >> 1]) && (mask >> key & 1u) != 0;
-          s[nt][e] = keep ? s[nt][e] * scale : -INFINITY;
+          s[nt][e] = (visible[e >> 1] >> key & 1u) != 0 ? s[nt][e] * scale : -INFINITY;
           top[e >> 1] = fmaxf(top[e >> 1], s[nt][e]);
         }
       bool moves = false;
@@ -429,6 +435,7 @@ __global__ void __launch_bounds__(SuffixSdpa<kDim>::kThreads, SuffixSdpa<kDim>::
       const int r = h == 0 ? r_low : r_high;
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (m[h] == -INFINITY && keyed[h] != 0) l[h] += 1.f;  // scores of -inf alone are keys all the same (or NaN, which l keeps)
       if (r < rows) {
         if ((lane & 3) == 0) __stcg(p.fragment_ml + at + r, make_float2(m[h], l[h]));
 #pragma unroll
@@ -498,20 +505,22 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         x[e] = e < here && active ? __ldcg(reinterpret_cast<const float4*>(o_at + (c0 + e) * step * kDim) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const uint32_t keyed = __ballot_sync(0xffffffffu, ml.x != -INFINITY || ml.y != 0.f);  // the partial results that have a key
+      if (keyed == 0) continue;
       float highest = ml.x;
 #pragma unroll
       for (int offset = 4; offset > 0; offset >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, offset));
       highest = __shfl_sync(0xffffffffu, highest, 0);
-      if (highest == -INFINITY) continue;  // (the same for the warp)
-      const float m_new = fmaxf(m, highest), keep = m == -INFINITY ? 0.f : exp2_approx(m - m_new);
+      // (what is the maximum itself counts once, -inf too: it still is one key or more if nothing higher comes)
+      const float m_new = fmaxf(m, highest), keep = m == m_new ? 1.f : exp2_approx(m - m_new);
       m = m_new;
-      const float weight = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - m);
+      const float weight = ml.x == m ? 1.f : exp2_approx(ml.x - m);
       l = l * keep + weight * ml.y;
       sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float w = __shfl_sync(0xffffffffu, weight, e);
-        if (w != 0.f)  // (a partial result without a key may hold anything)
+        if ((keyed >> e & 1u) != 0)  // (a partial result without a key may hold anything)
           sum.x = fmaf(w, x[e].x, sum.x), sum.y = fmaf(w, x[e].y, sum.y), sum.z = fmaf(w, x[e].z, sum.z), sum.w = fmaf(w, x[e].w, sum.w);
       }
     }
@@ -534,11 +543,10 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
     float highest = m;
 #pragma unroll
     for (int w = 1; w < kRowWarps; ++w) highest = fmaxf(highest, other_ml[w].x);
-    l = 0.f, sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    m = highest, l = 0.f, sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) {
-      const float weight = other_ml[w].x == -INFINITY ? 0.f : exp2_approx(other_ml[w].x - highest);
-      if (weight == 0.f) continue;
+      const float weight = other_ml[w].x == highest ? 1.f : exp2_approx(other_ml[w].x - highest);
       l += weight * other_ml[w].y;
       if (active) {
         const float4 x = other_sum[w][lane];
@@ -546,7 +554,7 @@ __global__ void __launch_bounds__(128) sdpa_merge_rows_kernel(const SuffixSdpaAr
       }
     }
   }
-  const float reciprocal = l == 0.f ? 0.f : 1.f / l;  // no key: zeros
+  const float reciprocal = l == 0.f ? 0.f : m == -INFINITY ? NAN : 1.f / l;  // no key: zeros; only keys whose score is -inf: 0 / 0
   if (there && active && lane * 4 < a.head_dim) {
     T* out = static_cast<T*>(a.out) + t * a.o_st + head * a.o_sh + lane * 4;
     *reinterpret_cast<uint2*>(out) = make_uint2(prefix_pack<T>(sum.x * reciprocal, sum.y * reciprocal), prefix_pack<T>(sum.z * reciprocal, sum.w * reciprocal));
