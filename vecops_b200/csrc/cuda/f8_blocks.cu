@@ -58,8 +58,11 @@ int32_t check_f8(const VecopsB200MatmulF8& p, VecopsError* error) {
   return VECOPS_STATUS_OK;
 }
 
-// Whether TMA can address both operands: contiguous along K, rows on 16-byte boundaries.
+// Whether TMA can address both operands: contiguous along K, rows on 16-byte boundaries; and whether the tiles' coordinates, which
+// reach past an extent by less than a tile, fit 32 bits.
 bool f8_addressable(const VecopsB200MatmulF8& p) {
+  constexpr int64_t kTiledLimit = kExtentLimit - 256;
+  if (p.m > kTiledLimit || p.n > kTiledLimit || p.k > kTiledLimit) return false;
   auto rows = [&](const void* base, int64_t count, int64_t stride, int64_t stride_k) {
     return (stride_k == 1 || p.k == 1) && decode_aligned(base, 16) && (count == 1 || (stride % 16 == 0 && stride >= p.k));
   };
@@ -71,7 +74,7 @@ constexpr int64_t kStreamRows = 128;  // rows of A the streaming kernel holds at
 int32_t select_f8(const VecopsB200MatmulF8& p, uint32_t* kernel, VecopsError* error) {
   const bool addressable = f8_addressable(p);
   if ((p.kernel == VECOPS_B200_F8_STREAM || p.kernel == VECOPS_B200_F8_TILED) && !addressable)
-    return set_error(error, VECOPS_STATUS_NOT_APPLICABLE, "matmul_f8: kernel %u needs operands contiguous along K on 16-byte aligned rows", p.kernel);
+    return set_error(error, VECOPS_STATUS_NOT_APPLICABLE, "matmul_f8: kernel %u needs operands contiguous along K on 16-byte aligned rows, and extents up to 2^31 - 256", p.kernel);
   if (p.kernel == VECOPS_B200_F8_STREAM && p.m > kStreamRows)
     return set_error(error, VECOPS_STATUS_NOT_APPLICABLE, "matmul_f8: the streaming kernel serves up to %lld rows, not %lld", (long long)kStreamRows, (long long)p.m);
   if (p.kernel != VECOPS_B200_F8_AUTO) *kernel = p.kernel;
