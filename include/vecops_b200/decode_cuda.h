@@ -176,6 +176,8 @@ typedef struct VecopsB200PrefixAttention {
   uint32_t reserved;
 } VecopsB200PrefixAttention;
 
+/* Scratch of a call: by the record's extents, whether it has query_starts, and the device's SM count - whatever the pointers, strides and
+ * contents are, so one size serves every call of a shape.  A call whose rows lie off 16-byte boundaries does without. */
 VECOPS_B200_EXPORT int32_t vecops_b200_prefix_sdpa_workspace(const VecopsB200PrefixAttention* attention, uint64_t* bytes, VecopsError* error);
 VECOPS_B200_EXPORT int32_t vecops_b200_prefix_sdpa_run(const VecopsB200PrefixAttention* attention, VecopsError* error);
 

@@ -119,17 +119,21 @@ struct PrefixPlan {
   uint64_t ml_at = 0, fragment_o_at = 0, fragment_ml_at = 0, sums_at = 0, total = 0;
 };
 
-PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
-  PrefixPlan p;
-  // sixteen-byte loads of every row
+// Whether every row of the operands can be loaded and stored in sixteen bytes.
+bool prefix_addressable(const VecopsB200PrefixAttention& a) {
   auto rows_ok = [](const void* base, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2) {
     return decode_aligned(base, 16) && (n0 <= 1 || s0 % 8 == 0) && (n1 <= 1 || s1 % 8 == 0) && (n2 <= 1 || s2 % 8 == 0);
   };
+  return rows_ok(a.q, a.tokens, a.q_stride_token, a.q_heads, a.q_stride_head, 1, 0) && rows_ok(a.out, a.tokens, a.out_stride_token, a.q_heads, a.out_stride_head, 1, 0) &&
+         rows_ok(a.k_cache, a.pages, a.k_stride_page, a.page_size, a.k_stride_slot, a.kv_heads, a.k_stride_head) &&
+         rows_ok(a.v_cache, a.pages, a.v_stride_page, a.page_size, a.v_stride_slot, a.kv_heads, a.v_stride_head);
+}
+
+// By the extents alone (and whether there are query_starts): what the scratch is sized by must not change with an address.
+PrefixPlan plan_prefix(const VecopsB200PrefixAttention& a, int sms) {
+  PrefixPlan p;
   const bool pages_ok = a.page_size % 128 == 0 || (a.page_size % 8 == 0 && 128 % a.page_size == 0);  // a tile of 128 keys is whole pages or lies in one
   p.fast = a.head_dim <= 128 && a.head_dim % 8 == 0 && (a.prefix_len == 0 || pages_ok) &&
-           rows_ok(a.q, a.tokens, a.q_stride_token, a.q_heads, a.q_stride_head, 1, 0) && rows_ok(a.out, a.tokens, a.out_stride_token, a.q_heads, a.out_stride_head, 1, 0) &&
-           rows_ok(a.k_cache, a.pages, a.k_stride_page, a.page_size, a.k_stride_slot, a.kv_heads, a.k_stride_head) &&
-           rows_ok(a.v_cache, a.pages, a.v_stride_page, a.page_size, a.v_stride_slot, a.kv_heads, a.v_stride_head) &&
            a.tokens * (a.q_heads / a.kv_heads) <= INT64_C(256) * 65535 &&  // (row blocks are a grid's third dimension)
            a.kv_heads <= 65535 && a.batch < (1 << 24) && a.tokens < (1 << 24);
   if (!p.fast) return p;
@@ -392,7 +396,7 @@ int32_t vecops_b200_prefix_sdpa_run(const VecopsB200PrefixAttention* attention, 
   DecodeDevice device;
   rc = decode_enter(a.device_index, &device, error);
   if (rc != VECOPS_STATUS_OK) return rc;
-  const PrefixPlan plan = plan_prefix(a, device.sms);
+  const PrefixPlan plan = prefix_addressable(a) ? plan_prefix(a, device.sms) : PrefixPlan{};
   if (plan.total != 0 && (a.workspace == nullptr || !decode_aligned(a.workspace, 256) || a.workspace_size < plan.total))
     return set_error(error, VECOPS_STATUS_INVALID_ARGUMENT, "prefix_sdpa needs %llu bytes of 256-byte aligned device scratch (vecops_b200_prefix_sdpa_workspace)",
                      (unsigned long long)plan.total);
