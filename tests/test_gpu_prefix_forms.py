@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from tests import decode_reference as ref
-from tests.test_gpu_decode import BF16, F16, on_device, ops, prefix_inputs  # noqa: F401  (ops is a fixture)
+from tests.test_gpu_decode import (BF16, F16, check_step, decode_step, on_device, ops, prefix_inputs,  # noqa: F401  (ops is a fixture)
+                                   step_state, step_tables)
 from vecops_b200 import capi
 
 pytestmark = pytest.mark.gpu
@@ -139,3 +140,190 @@ def test_scores_of_minus_infinity(ops, case):  # noqa: F811
     assert out.isnan().all()
     at([shared[-1:]], float("inf"))
     assert attend(ops, on_device(inputs), form).isnan().all()
+
+
+# ------------------------------------------------------------------------------------------------ the prefix kernel: operands, streams, graphs
+
+# both row blocks; few rows and 128 dims; few rows and 64 dims in chunks of five tiles
+SHAPES = [(40, 8, 2, 128, 3000), (20, 8, 8, 128, 896), (5, 48, 48, 64, 1152)]
+
+
+def shape_inputs(shape, seed, page=16, **more):
+    batch, hq, hkv, d, prefix = shape
+    return prefix_inputs([1] * batch, [1 + 7 * i % 41 for i in range(batch)], prefix, hq, hkv, d, page, BF16, seed, **{"ragged": False, "width": 3, **more})
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_the_prefix_kernel_takes_strided_operands(ops, shape):  # noqa: F811
+    batch, hq, hkv, d, _ = shape
+    inputs = shape_inputs(shape, 61)
+    device = on_device(inputs)
+    want = ref.prefix_attention(**inputs)
+    q = torch.zeros(batch, hq, 3, d, dtype=BF16, device="cuda")
+    q[:, :, 1] = device["q"]
+    heads_first = [device[name].transpose(1, 2).contiguous().transpose(1, 2) for name in ("k_cache", "v_cache")]
+    both = torch.stack([device["k_cache"], device["v_cache"]], dim=3)  # a key beside its value
+    wide = torch.full((batch, 9), -1, dtype=torch.int32, device="cuda")
+    wide[:, :3] = device["page_table"]
+    for change in (dict(q=q[:, :, 1]), dict(k_cache=heads_first[0], v_cache=heads_first[1]), dict(k_cache=both[:, :, :, 0], v_cache=both[:, :, :, 1]),
+                   dict(page_table=wide[:, :3])):
+        ref.assert_within(attend(ops, {**device, **change}, PREFIX_KERNEL), *want)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
+def test_the_prefix_kernel_scales(ops, shape, scale):  # noqa: F811
+    inputs = shape_inputs(shape, 62, scale=scale)
+    ref.assert_within(attend(ops, on_device(inputs), PREFIX_KERNEL), *ref.prefix_attention(**inputs))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_the_prefix_kernel_drops_absent_pages_and_never_uses_what_lies_behind_the_keys(ops, shape):  # noqa: F811
+    page = 16
+    inputs = shape_inputs((*shape[:-1], shape[-1] - 5), 63)  # ends inside a page
+    pages = inputs["k_cache"].shape[0]
+    inputs["prefix_pages"][1], inputs["prefix_pages"][2] = pages, -7
+    inputs["prefix_pages"][8:16] = -1  # a whole tile of 128 keys
+    inputs["lengths"][1] = -1
+    used = torch.zeros(inputs["k_cache"].shape[:2], dtype=torch.bool)
+    for j in range(inputs["prefix_len"]):
+        at = int(inputs["prefix_pages"][j // page])
+        if 0 <= at < pages:
+            used[at, j % page] = True
+    for b, length in enumerate(inputs["lengths"].tolist()):
+        for j in range(max(0, length)):
+            used[inputs["page_table"][b, j // page], j % page] = True
+    for name in ("k_cache", "v_cache"):
+        inputs[name][~used] = float("nan")
+    ref.assert_within(attend(ops, on_device(inputs), PREFIX_KERNEL), *ref.prefix_attention(**inputs))
+
+
+def test_the_prefix_kernel_reads_far_into_a_long_cache(ops):  # noqa: F811
+    pages, page, hkv, d = (1 << 20) + 3, 16, 2, 128  # 8 GiB a cache, element offsets past 2^32
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB of device memory")
+    inputs = shape_inputs((40, 8, hkv, d, 3000), 64)
+    small = inputs["k_cache"].shape[0]
+    far = pages - small + torch.arange(small, dtype=torch.int64)
+    device = on_device(inputs)
+    for name in ("k_cache", "v_cache"):
+        cache = torch.zeros(pages, page, hkv, d, dtype=BF16, device="cuda")
+        cache[far.cuda()] = device[name]
+        device[name] = cache
+    for name in ("prefix_pages", "page_table"):
+        device[name] = far[inputs[name].long()].int().cuda()
+    ref.assert_within(attend(ops, device, PREFIX_KERNEL), *ref.prefix_attention(**inputs))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_prefix_kernels_on_two_streams_at_once_repeat_bit_for_bit(ops, shape):  # noqa: F811
+    states = [on_device(shape_inputs(shape, seed)) for seed in (65, 66)]
+    want = [attend(ops, state, PREFIX_KERNEL).clone() for state in states]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    results = [[], []]
+    for _ in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                results[i].append(attend(ops, states[i], PREFIX_KERNEL))
+    torch.cuda.synchronize()
+    graphs = []
+    for stream, state in zip(streams, states):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = [attend(ops, state, PREFIX_KERNEL) for _ in range(3)]  # one call's kernels start under the one before
+        graphs.append((graph, out))
+    for _ in range(5):
+        for stream, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in [*results[i], *graphs[i][1]]:
+            assert torch.equal(out, want[i])
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_captured_prefix_kernel_follows_its_tensors(ops, shape):  # noqa: F811
+    static = on_device(shape_inputs(shape, 67))
+    attend(ops, static, PREFIX_KERNEL)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend(ops, static, PREFIX_KERNEL)
+    for seed in (68, 69):
+        inputs = shape_inputs(shape, seed)
+        inputs["lengths"] = (inputs["lengths"] * seed) % 49 - 1  # padding and empty suffixes among them
+        for name, tensor in inputs.items():
+            if isinstance(tensor, torch.Tensor):
+                static[name].copy_(tensor)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.assert_within(out, *ref.prefix_attention(**inputs))
+        assert torch.equal(out, attend(ops, static, PREFIX_KERNEL))
+    del graph
+
+
+@pytest.mark.parametrize("batch,hq,hkv,d,prefix", [(40, 8, 2, 128, 3000), (20, 8, 8, 64, 1152)])
+def test_a_decode_step_over_the_prefix_kernel_eager_and_captured(ops, batch, hq, hkv, d, prefix):  # noqa: F811
+    hidden = 512
+    weights, inputs, table = step_state(ops, batch, hidden, hq, hkv, d, 16, prefix, 71)
+    k_cache, v_cache = inputs["k_cache"].cuda(), inputs["v_cache"].cuda()
+    static = list(step_tables(inputs, table, 0, batch))
+    x = torch.zeros(batch, hidden, dtype=BF16, device="cuda")
+    before = capi.library().vecops_b200_launch_count()
+    decode_step(ops, x, weights, k_cache.clone(), v_cache.clone(), static, hq, hkv, d)
+    assert capi.library().vecops_b200_launch_count() - before == 5 + PREFIX_KERNEL
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = decode_step(ops, x, weights, k_cache, v_cache, static, hq, hkv, d)
+    eager_k, eager_v = inputs["k_cache"].cuda(), inputs["v_cache"].cuda()
+    for step in range(2):
+        tables = step_tables(inputs, table, 7 * step + 3, batch, padding=step)
+        x.copy_(torch.randn(batch, hidden, generator=torch.Generator().manual_seed(step)).to(BF16))
+        earlier = eager_k.cpu(), eager_v.cpu()
+        result = decode_step(ops, x, weights, eager_k, eager_v, tables, hq, hkv, d)
+        check_step(x, weights, earlier, (eager_k.cpu(), eager_v.cpu()), tables, result, hq, hkv, d)
+        for old, new in zip(static, tables):
+            if isinstance(old, torch.Tensor):
+                old.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        for mine, theirs in zip(captured, result):
+            assert torch.equal(mine, theirs)
+        assert torch.equal(k_cache, eager_k) and torch.equal(v_cache, eager_v)
+    del graph
+
+
+def test_branches_of_a_captured_graph_join_at_the_prefix_kernel(ops):  # noqa: F811
+    # a product on one branch, attention on the other, a product and attention behind both
+    inputs = on_device(shape_inputs((40, 4, 2, 128, 3000), 72))
+    g = torch.Generator().manual_seed(73)
+    x = torch.randn(40, 512, generator=g).to(BF16).cuda()
+    w, w_scale = ops.quantize_blocks(torch.randn(512, 512, generator=g).to(BF16).cuda(), 128)
+    side = torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            y = ops.matmul_f8_blocks(*ops.quantize_blocks(x, 1), w, w_scale, BF16)
+        o = attend(ops, inputs, PREFIX_KERNEL)
+        here.wait_stream(side)
+        z = ops.matmul_f8_blocks(*ops.quantize_blocks(o.view(40, 512) + y, 1), w, w_scale, BF16)
+        return y, o, z, attend(ops, dict(inputs, q=z.view(40, 4, 128)), PREFIX_KERNEL)
+
+    want = [r.clone() for r in run()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        for r in got:
+            r.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for r, e in zip(got, want):
+            assert torch.equal(r, e)
+    del graph
