@@ -327,3 +327,22 @@ def test_branches_of_a_captured_graph_join_at_the_prefix_kernel(ops):  # noqa: F
         for r, e in zip(got, want):
             assert torch.equal(r, e)
     del graph
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_caches_whose_heads_or_pages_share_memory(ops, shape):  # noqa: F811
+    hkv = shape[2]
+    inputs = shape_inputs(shape, 81)
+    one = {name: inputs[name][:, :, :1].contiguous() for name in ("k_cache", "v_cache")}
+    device = on_device(inputs)
+    shared = {name: cache.cuda().expand(-1, -1, hkv, -1) for name, cache in one.items()}
+    # one head's keys, values or both for all heads
+    for names in (("k_cache",), ("v_cache",), ("k_cache", "v_cache")):
+        want = ref.prefix_attention(**{**inputs, **{name: one[name].expand(-1, -1, hkv, -1) for name in names}})
+        ref.assert_within(attend(ops, {**device, **{name: shared[name] for name in names}}, PREFIX_KERNEL), *want)
+    # one page for all, one key for all of a page's: left to the simple kernel
+    pages, page = inputs["k_cache"].shape[:2]
+    for name, few in (("k_cache", inputs["k_cache"][:1].expand(pages, -1, -1, -1)), ("v_cache", inputs["v_cache"][:, :1].expand(-1, page, -1, -1))):
+        on_gpu = device[name][:1].expand(pages, -1, -1, -1) if name == "k_cache" else device[name][:, :1].expand(-1, page, -1, -1)
+        assert 0 in on_gpu.stride()
+        ref.assert_within(attend(ops, {**device, name: on_gpu}, SIMPLE), *ref.prefix_attention(**{**inputs, name: few}))

@@ -119,14 +119,16 @@ struct PrefixPlan {
   uint64_t ml_at = 0, fragment_o_at = 0, fragment_ml_at = 0, sums_at = 0, total = 0;
 };
 
-// Whether every row of the operands can be loaded and stored in sixteen bytes.
+// Whether every row of the operands can be loaded and stored in sixteen bytes, and the caches' pages be addressed by TMA (whose strides are
+// not 0; heads that share their rows are one head to it).
 bool prefix_addressable(const VecopsB200PrefixAttention& a) {
   auto rows_ok = [](const void* base, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2) {
     return decode_aligned(base, 16) && (n0 <= 1 || s0 % 8 == 0) && (n1 <= 1 || s1 % 8 == 0) && (n2 <= 1 || s2 % 8 == 0);
   };
   return rows_ok(a.q, a.tokens, a.q_stride_token, a.q_heads, a.q_stride_head, 1, 0) && rows_ok(a.out, a.tokens, a.out_stride_token, a.q_heads, a.out_stride_head, 1, 0) &&
          rows_ok(a.k_cache, a.pages, a.k_stride_page, a.page_size, a.k_stride_slot, a.kv_heads, a.k_stride_head) &&
-         rows_ok(a.v_cache, a.pages, a.v_stride_page, a.page_size, a.v_stride_slot, a.kv_heads, a.v_stride_head);
+         rows_ok(a.v_cache, a.pages, a.v_stride_page, a.page_size, a.v_stride_slot, a.kv_heads, a.v_stride_head) &&
+         (a.pages <= 1 || (a.k_stride_page > 0 && a.v_stride_page > 0)) && (a.page_size <= 1 || (a.k_stride_slot > 0 && a.v_stride_slot > 0));
 }
 
 // By the extents alone (and whether there are query_starts): what the scratch is sized by must not change with an address.
@@ -255,18 +257,20 @@ int32_t run_prefix(const VecopsB200PrefixAttention& a, const PrefixPlan& plan, c
     p.box_keys = static_cast<int>(a.page_size < 128 ? a.page_size : 128);
     p.partial_o = partial_o, p.partial_ml = partial_ml, p.status = device.status;
     CUtensorMap map_k, map_v;
-    auto cache_map = [&](CUtensorMap* map, const void* base, int64_t page, int64_t slot, int64_t head) {
+    auto cache_map = [&](CUtensorMap* map, const void* base, int64_t page, int64_t slot, int64_t head, int* head_step) {
+      *head_step = head > 0 ? 1 : 0;
       // (a dimension of one has no stride that matters, but the map wants a legal one)
       auto bytes = [](int64_t n, int64_t stride) { return static_cast<uint64_t>(n > 1 ? stride * 2 : 16); };
-      const uint64_t dims[4] = {static_cast<uint64_t>(a.head_dim), static_cast<uint64_t>(a.page_size), static_cast<uint64_t>(a.kv_heads), static_cast<uint64_t>(a.pages)};
-      const uint64_t strides[3] = {bytes(a.page_size, slot), bytes(a.kv_heads, head), bytes(a.pages, page)};
+      const uint64_t dims[4] = {static_cast<uint64_t>(a.head_dim), static_cast<uint64_t>(a.page_size), static_cast<uint64_t>(head > 0 ? a.kv_heads : 1),
+                                static_cast<uint64_t>(a.pages)};
+      const uint64_t strides[3] = {bytes(a.page_size, slot), bytes(static_cast<int64_t>(dims[2]), head), bytes(a.pages, page)};
       const uint32_t box[4] = {64, static_cast<uint32_t>(p.box_keys), 1, 1};
       const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
       return shim_encode_map(map, type, 4, base, dims, strides, box, error);
     };
-    int32_t rc = cache_map(&map_k, a.k_cache, a.k_stride_page, a.k_stride_slot, a.k_stride_head);
+    int32_t rc = cache_map(&map_k, a.k_cache, a.k_stride_page, a.k_stride_slot, a.k_stride_head, &p.k_head_step);
     if (rc != VECOPS_STATUS_OK) return rc;
-    rc = cache_map(&map_v, a.v_cache, a.v_stride_page, a.v_stride_slot, a.v_stride_head);
+    rc = cache_map(&map_v, a.v_cache, a.v_stride_page, a.v_stride_slot, a.v_stride_head, &p.v_head_step);
     if (rc != VECOPS_STATUS_OK) return rc;
     config.gridDim = dim3(static_cast<unsigned>(plan.chunks), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(plan.row_blocks));
     config.blockDim = dim3(G::kThreads);

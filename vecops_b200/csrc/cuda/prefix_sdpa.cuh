@@ -78,6 +78,7 @@ struct PrefixTcArgs {
   int tiles, tiles_per_chunk;
   int both_rows;       // 1: the groups hold two blocks of 128 rows; 0: one block, the groups take the key tiles in turn
   int box_keys;        // keys per TMA box: min(page_size, 128)
+  int k_head_step, v_head_step;  // from head to head in the maps: 1, or 0 when all heads have the same rows
   float* partial_o;    // [record][kv head][row][kDim]
   float2* partial_ml;  // [record][kv head][row] (m, l); (-inf, 0) for no key, (-inf, > 0) for keys whose scores are all -inf
   uint32_t* status;
@@ -202,11 +203,11 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     auto mine = [&](int tile) { return lane < boxes && tile < n && key_of(tile) < p.a.prefix_len; };
     auto page_of = [&](int tile) { return mine(tile) ? __ldg(p.a.prefix_pages + key_of(tile) / p.a.page_size) : -1; };
     auto bytes_of = [&](int tile) { return __popc(__ballot_sync(0xffffffffu, mine(tile))) * p.box_keys * 128 * G::kAtoms; };
-    auto load = [&](const CUtensorMap* map, int tile, int page, uint32_t to, uint32_t bar) {
+    auto load = [&](const CUtensorMap* map, int tile, int head, int page, uint32_t to, uint32_t bar) {
       if (mine(tile)) {
 #pragma unroll
         for (int atom = 0; atom < G::kAtoms; ++atom)  // a page outside the cache reads as zeros
-          tma_load_4d(to + atom * G::kAtomBytes + lane * p.box_keys * 128, map, bar, atom * 64, key_of(tile) % p.a.page_size, kv, page);
+          tma_load_4d(to + atom * G::kAtomBytes + lane * p.box_keys * 128, map, bar, atom * 64, key_of(tile) % p.a.page_size, head, page);
       }
     };
     int ahead[2] = {page_of(0), page_of(1)};  // of the next K tiles, looked up before they are needed
@@ -230,8 +231,8 @@ prefix_sdpa_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         mbar_arrive_expect_tx(bar, bytes);
       }
       __syncwarp();
-      if (v_tile >= 0) load(&map_v, v_tile, v_page, to, bar);
-      if (k_tile < n) load(&map_k, k_tile, k_page, to + G::kTileBytes, bar);
+      if (v_tile >= 0) load(&map_v, v_tile, kv * p.v_head_step, v_page, to, bar);
+      if (k_tile < n) load(&map_k, k_tile, kv * p.k_head_step, k_page, to + G::kTileBytes, bar);
       if (++slot == steps) slot = 0, phase ^= 1u;
     }
   } else if (warp == 1) {
