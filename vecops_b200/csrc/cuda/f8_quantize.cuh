@@ -33,21 +33,11 @@ __device__ __forceinline__ float f8_source<__nv_bfloat16>(__nv_bfloat16 x) { ret
 template <>
 __device__ __forceinline__ float f8_source<__half>(__half x) { return __half2float(x); }
 
-// Eight consecutive elements of a row from column `col`; what lies past `cols` reads as zero.  kVec: the row starts on a
-// 16-byte boundary and is contiguous, so eight elements that are all there come in 16-byte loads.
-template <typename T, bool kVec>
+// Eight neighbouring elements of a row of any stride from column `col` on; what lies past `cols` reads as zero.
+template <typename T>
 __device__ __forceinline__ void f8_load8(const T* row, long long stride_col, long long col, long long cols, float (&x)[8]) {
-  if (kVec && col + 8 <= cols) {
-    uint4 raw[sizeof(T) / 2];
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(row + col) + i);
-    const T* values = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = f8_source(values[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = col + e < cols ? f8_source(row[(col + e) * stride_col]) : 0.f;
-  }
+  for (int e = 0; e < 8; ++e) x[e] = col + e < cols ? f8_source(row[(col + e) * stride_col]) : 0.f;
 }
 
 __device__ __forceinline__ float f8_block_amax(const float (&x)[8], float amax) {
@@ -58,19 +48,14 @@ __device__ __forceinline__ float f8_block_amax(const float (&x)[8], float amax) 
 
 __device__ __forceinline__ float f8_bounded_amax(float amax) { return fminf(fmaxf(amax, F8Quantize::kAmaxFloor), FLT_MAX); }
 
-template <bool kVec>
 __device__ __forceinline__ void f8_store8(uint8_t* row, long long col, long long cols, const float (&x)[8], float factor) {
   uint16_t pairs[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     pairs[e] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * e] * factor, x[2 * e + 1] * factor), __NV_SATFINITE, __NV_E4M3);
-  if (kVec && col + 8 <= cols) {
-    *reinterpret_cast<uint2*>(row + col) = make_uint2(pairs[0] | (static_cast<uint32_t>(pairs[1]) << 16), pairs[2] | (static_cast<uint32_t>(pairs[3]) << 16));
-  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (col + e < cols) row[col + e] = static_cast<uint8_t>(pairs[e >> 1] >> (8 * (e & 1)));
-  }
+  for (int e = 0; e < 8; ++e)
+    if (col + e < cols) row[col + e] = static_cast<uint8_t>(pairs[e >> 1] >> (8 * (e & 1)));
 }
 
 struct F8QuantizeArgs {
@@ -268,13 +253,13 @@ __global__ void __launch_bounds__(256) f8_quantize_strided_kernel(const F8Quanti
     const long long row = block / col_blocks, col_block = block - row * col_blocks;
     const long long col = col_block * F8Quantize::kBlock + lane * 8;
     float x[8];
-    f8_load8<T, false>(static_cast<const T*>(p.src) + row * p.src_sr, p.src_sc, col, p.cols, x);
+    f8_load8(static_cast<const T*>(p.src) + row * p.src_sr, p.src_sc, col, p.cols, x);
     float amax = f8_block_amax(x, 0.f);
     const unsigned members = 0xffffu << (threadIdx.x & 16);  // the other half of the warp may be done
 #pragma unroll
     for (int offset = 8; offset > 0; offset >>= 1) amax = fmaxf(amax, __shfl_xor_sync(members, amax, offset));
     amax = f8_bounded_amax(amax);
-    f8_store8<false>(p.dst + row * p.dst_sr, col, p.cols, x, F8Quantize::kMax / amax);
+    f8_store8(p.dst + row * p.dst_sr, col, p.cols, x, F8Quantize::kMax / amax);
     if (lane == 0) p.scale[row * p.scale_sr + col_block * p.scale_sc] = amax / F8Quantize::kMax;
   }
 }
