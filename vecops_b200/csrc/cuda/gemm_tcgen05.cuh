@@ -59,6 +59,10 @@
 
 namespace vb200 {
 
+// How a tile leaves: by each row's own thread, in 128-byte pieces by TMA, by stores to a multicast address, or by TMA but for pieces that
+// the end of a row cuts.  (TMA clips a row to whole 16 bytes, not to elements: where N is no multiple of that, it would write zeros behind it.)
+enum GemmStore : int { kStoreDirect = 0, kStoreTma = 1, kStoreMulticast = 2, kStoreTmaWhole = 3 };
+
 struct GemmTc {
   static constexpr int kBlockM = 128;
   static constexpr int kBlockN = 256;
@@ -322,7 +326,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_cons
     mbar_fence_init();
     tma_prefetch_descriptor(&tma_a);
     tma_prefetch_descriptor(&tma_b);
-    if (use_tma_store == 1) tma_prefetch_descriptor(&tma_c.map[0]);
+    if ((use_tma_store & 1) != 0) tma_prefetch_descriptor(&tma_c.map[0]);
   }
   if (warp == 1) {
     if constexpr (kPair) {
@@ -716,7 +720,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_cons
             words[16 + j] = pack_out16x2<OutT>(__uint_as_float(v1[2 * j]), __uint_as_float(v1[2 * j + 1]));
           }
         }
-        if (use_tma_store == 2) {
+        if (use_tma_store == kStoreMulticast) {
           // Multicast gather: stage the 32-row x 128-byte slab as for a TMA store, then read it back four rows at a
           // time - eight lanes per row, 16 bytes per lane, 128 contiguous bytes per row on the wire - and store to the
           // multicast address of the full result.  (`c` is that address, `ldc` the full result's pitch.)
@@ -743,7 +747,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_cons
               multimem_st_v4(c + static_cast<long long>(row0 + r) * ldc + c_col_offset + chunk_col, piece);
           }
           buf_sel ^= 1;
-        } else if (use_tma_store) {
+        } else if (use_tma_store == kStoreTma || (use_tma_store == kStoreTmaWhole && col0 + kOutCols <= N)) {
           const uint32_t buf = my_buf + buf_sel * G::kEpiBufBytes;
           // the store issued two slabs ago from this buffer must have read it
           if (lane == 0) tma_store_wait_read<1>();
@@ -802,7 +806,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_cons
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }
-    if (use_tma_store == 1 && lane == 0) tma_store_wait_all<0>();
+    if ((use_tma_store & 1) != 0 && lane == 0) tma_store_wait_all<0>();
     if (warp == 2 && lane == 0) {
       mark(15);
       if (trace != nullptr) trace[blockIdx.x * 16 + 14] = static_cast<unsigned long long>(clock64());  // ... and at the end

@@ -613,11 +613,13 @@ int32_t launch_tcgen05(const VecopsB200Matmul& p, const DeviceState& dev, cudaSt
   long long ldc = p.c_stride_m;
   int m = static_cast<int>(p.m), n = static_cast<int>(p.n), k = static_cast<int>(p.k);
   const float* scale = std::is_same<OutT, int32_t>::value ? nullptr : p.column_scale;
-  int store_flag = tma_store ? 1 : 0;
+  int store_flag = tma_store ? kStoreTma : kStoreDirect;
   if (gather.count > 0 && gather.multicast) {
     c = static_cast<OutT*>(gather.c[0]);
     ldc = gather.ldc;
-    store_flag = 2;
+    store_flag = kStoreMulticast;
+  } else if (gather.count == 0 && tma_store && p.n * sizeof(OutT) % 16 != 0) {
+    store_flag = kStoreTmaWhole;
   }
   // Row-tiles that share a sweep over N: as many as keep their rows of A (about 32 MB) in L2 while B streams past.
   long long group_tiles = G::kGroupBytes / (static_cast<long long>(mma_m) * p.k * static_cast<long long>(elem));
@@ -892,7 +894,8 @@ int32_t launch_w8_mixed(const VecopsB200Matmul& p, const DeviceState& dev, cudaS
   long long ldc = p.c_stride_m;
   int m = static_cast<int>(p.m), n = static_cast<int>(p.n), k = static_cast<int>(p.k);
   const float* scale = p.column_scale;
-  int store_flag = tma_store ? 1 : 0, num_dest = 1, col_offset = 0, raster_group = 4;
+  int store_flag = !tma_store ? kStoreDirect : p.n * sizeof(OutT) % 16 == 0 ? kStoreTma : kStoreTmaWhole;
+  int num_dest = 1, col_offset = 0, raster_group = 4;
   unsigned long long nonce = split > 1 ? fresh_nonce(p.workspace) : 0ull;
   uint32_t* status_word = status_word_of(device);
   unsigned long long* trace = g_trace;
