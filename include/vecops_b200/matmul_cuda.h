@@ -240,7 +240,8 @@ VECOPS_B200_EXPORT int32_t vecops_b200_take_device_status(int32_t device_index, 
  * ignored.  Each finished 32 x 128-byte piece of the slab is TMA-stored from shared memory straight into
  * columns [col0, col0 + n) of EVERY destination in `c` - the full [M, n_total] result of each GPU, own
  * included, reached through peer pointers (CUDA IPC / symmetric memory) - while the main loop continues.
- * Only stores cross GPUs.  The caller orders ranks afterwards (a barrier on the stream) before anyone reads. */
+ * A slab whose n is not a multiple of 16 bytes gets up to 15 bytes of zeros behind each row of it: room that no other
+ * slab has, as col0 is a multiple of 16 bytes.  Only stores cross GPUs.  The caller orders ranks afterwards (a barrier on the stream) before anyone reads. */
 typedef struct VecopsB200Gather {
   uint32_t struct_size;
   int32_t world;       /* number of destinations, 1..8 */

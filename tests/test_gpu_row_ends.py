@@ -34,3 +34,21 @@ def test_rows_that_end_off_boundaries_leave_what_follows(ops, a_type, b_type, c_
     ops.matmul_out(a, b, whole[:, :n], scale)
     assert torch.equal(whole[:, :n], plain)
     assert (whole[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n,col0", [(504, 0), (504, 504), (40, 768), (300, 64)])
+def test_a_gathered_slab_ends_with_its_own_columns(ops, dtype, n, col0):
+    # a slab that is no whole number of 128-byte pieces: the next rank's columns, which start right behind it, are another kernel's to write
+    from vecops_b200 import sharding
+    m, k, n_total = 200, 256, 1536
+    a, b = operand((m, k), BF16, 5), operand((n, k), BF16, 6)
+    full = [torch.full((m, n_total), -3.0, dtype=dtype, device="cuda") for _ in range(2)]
+    gemm = sharding.FusedGatherGemm(a, b, [t.data_ptr() for t in full], n_total, n_total, col0, dtype)
+    gemm.launch()
+    torch.cuda.synchronize()
+    want = ops.matmul(a, b, out_dtype=dtype)
+    end = col0 + -(-n // (16 // want.element_size())) * (16 // want.element_size())
+    for t in full:
+        assert torch.equal(t[:, col0:col0 + n], want)
+        assert (t[:, :col0] == -3).all() and (t[:, end:] == -3).all()

@@ -445,7 +445,6 @@ Tcgen05Plan plan_tcgen05(const VecopsB200Matmul& p, bool int8, size_t out_elem, 
 struct GatherTargets {
   int count = 0;                 // 0 = plain GEMM into p.c
   void* const* c = nullptr;      // `count` device pointers: each GPU's full C (own included)
-  int64_t n_total = 0;           // columns of the full C
   int64_t ldc = 0;               // row pitch of the full C, elements
   int64_t col0 = 0;              // first column of this rank's slab
   bool multicast = false;        // c[0] is the NVSwitch multicast address of the full C: multimem stores, no tensor map
@@ -532,12 +531,12 @@ int32_t launch_tcgen05(const VecopsB200Matmul& p, const DeviceState& dev, cudaSt
     col_offset = static_cast<int>(gather.col0);
     for (int d = 0; d < GemmStoreMaps::kMax; ++d) maps.map[d] = map_a;  // never dereferenced
   } else if (gather.count > 0) {
-    // every destination is a full [M, n_total] matrix; this rank's tiles land at column col0 + ...
+    // every destination is a full [M, n_total] matrix; this rank's tiles land at column col0 + ... and end, clipped by the map, with its slab
     tma_store = true;
     num_dest = gather.count;
     col_offset = static_cast<int>(gather.col0);
     for (int d = 0; d < gather.count; ++d) {
-      rc = make_map_2d(&maps.map[d], out_type, sizeof(OutT), gather.c[d], gather.n_total, p.m, gather.ldc * sizeof(OutT),
+      rc = make_map_2d(&maps.map[d], out_type, sizeof(OutT), gather.c[d], gather.col0 + p.n, p.m, gather.ldc * sizeof(OutT),
                        128 / sizeof(OutT), 32, error);
       if (rc != VECOPS_STATUS_OK) return rc;
     }
@@ -1544,7 +1543,6 @@ int32_t vecops_b200_matmul_allgather_run(const VecopsB200Matmul* problem, const 
     GatherTargets targets;
     targets.count = gather->world;
     targets.c = gather->c;
-    targets.n_total = gather->n_total;
     targets.ldc = gather->ldc;
     targets.col0 = gather->col0;
     targets.multicast = multicast;
