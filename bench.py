@@ -9,7 +9,7 @@ own epilogue, or by copies that run behind the next step's GEMM, whichever a ten
 (`--gather`; the trial times are in the line) - strong scaling, so the per-N values form one curve.  It fits one GPU (2.9 GB), where the slab is the
 whole result.  At N = 1 the other single-GPU configurations (BF16 4096^3, FP32 1024^3, INT8 4096x14336x4096, the three
 weight-only decode shapes) are measured too and reported under "configs", each with its own `roofline`,
-`cpu_baseline` and `e2e` record.
+`cpu_baseline` and `e2e` record (their figures; the same records with what they say in words go to stderr).
 
 A step is one pass of the operator over one batch of synthetic input.  `value` is measured with the operands
 resident in HBM (CUDA events on the launching stream, max over ranks); `e2e` runs the same step through the
@@ -1197,7 +1197,7 @@ def run_ours(args) -> None:
                 except Exception as error:  # noqa: BLE001
                     configs[extra] = {"error": repr(error)}
                 torch.cuda.empty_cache()
-            line["configs"] = configs
+            line["configs"] = brief(configs)
             extras = {}
             for key, measure in [
                     ("c2_bf16_4096_fused_bias_silu", lambda: measure_single("c2_bf16_4096", 50, 5, dev, port, peaks, peak_source, fused=True)),
@@ -1210,11 +1210,22 @@ def run_ours(args) -> None:
                 except Exception as error:  # noqa: BLE001
                     extras[key] = {"error": repr(error)}
                 torch.cuda.empty_cache()
-            line["next_rows"] = extras
+            line["next_rows"] = brief(extras)
+            # what the records say in words is more than half of them, and stays out of the line
+            print("[bench] records in full: " + json.dumps({"configs": configs, "next_rows": extras}), file=sys.stderr, flush=True)
     if rank == 0:
         print(json.dumps(line), flush=True)
     if world > 1:
         dist.destroy_process_group()
+
+
+def brief(record):
+    """A record without its prose, its figures to six digits."""
+    if isinstance(record, dict):
+        return {key: brief(value) for key, value in record.items() if key == "error" or not (isinstance(value, str) and len(value) > 32)}
+    if isinstance(record, list):
+        return [brief(value) for value in record]
+    return float(f"{record:.6g}") if isinstance(record, float) else record
 
 
 def measure_e2e_sharded(w, o, host_inputs, step_launch, full, n0: int, n1: int, steps: int, warmup: int, dev, a_peers=None) -> dict:
