@@ -55,8 +55,9 @@ VECOPS_B200_EXPORT int32_t vecops_b200_quantize_blocks(const VecopsB200QuantizeB
  *
  *     C[m,n] = sum_b a_scale[m,b] * b_scale[n / 128, b] * sum_{k in block b} A[m,k] * B[n,k]        (blocks of 128 along K)
  *
- * Each block's sum is accumulated in fp32 and enters the total in fp32 with its scale; one rounding to C's type.  K == 0
- * stores zeros. */
+ * Each block's sum is accumulated in fp32 and enters the total in fp32 with its scale; one rounding to C's type.  The two scales
+ * are multiplied with each other first: where that product leaves fp32's normal range, 2^-126 to 2^128, a block's share loses digits or
+ * becomes inf, or NaN beside a sum of 0.  K == 0 stores zeros. */
 typedef enum VecopsB200MatmulF8Kernel {
   VECOPS_B200_F8_AUTO = 0,
   VECOPS_B200_F8_GENERIC = 1, /* CUDA cores; any strides */
@@ -141,6 +142,10 @@ VECOPS_B200_EXPORT int32_t vecops_b200_cache_append(const VecopsB200CacheAppend*
  * so on.  Query head h reads key/value head h / (q_heads / kv_heads).
  *
  *     out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q.k_j - max)      over prefix keys [0, prefix_len) and the seen suffix keys
+ *
+ * Scores, maxima, both sums and the result before its one rounding are fp32; in the first sum the kernels on the tensor cores round p_j to q's
+ * type, which a 16-bit product takes (the second keeps all of it): an error of half a step a key, under the rounding of the result
+ * where many keys have weight.
  *
  * Prefix key j lies in page prefix_pages[j / page_size], suffix key j of sequence b in page page_table[b][j / page_size].
  * Keys of a page number outside [0, pages) count as absent, as do suffix keys past the table's width.  A query that sees

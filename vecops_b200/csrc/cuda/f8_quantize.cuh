@@ -4,7 +4,8 @@
 //
 // One division per block and one multiplication per element: x * (448 / amax) differs from x / scale by at most
 // 1.5 fp32 roundings, 2^13 times finer than an e4m3 step.  Memory bound: an element is read once and one byte written.
-// Measured at 4096 x 14336 bf16 (178 MB): 32 us for 1 x 128 blocks, 33.5 us for 128 x 128, 5.5 and 5.3 TB/s.  Rows off 16-byte
+// Measured at 4096 x 14336 bf16 (178 MB): 32 us for 1 x 128 blocks, 33.5 us for 128 x 128, 5.5 and 5.3 TB/s; fp32 (295 MB): 46 and 59
+// us, 6.4 and 5.0 TB/s (a CTA of the tile kernel holds twice the registers, so fewer of them load at once).  Rows off 16-byte
 // boundaries, 1322 x 12485 bf16 (50 MB): 15.3 and 17 us, 3.2 and 2.9 TB/s; by the kernel for any strides 32 us.
 #pragma once
 

@@ -9,7 +9,8 @@
 // item's (tcgen05's 128 would be nearly empty).  Warps share nothing and meet at no barrier.  Each runs m' = max(m, s), l, O over its part of an item and leaves them as a fragment;
 // sdpa_merge_rows_kernel, launched behind, joins a row's fragments and its prefix records,
 //     M = max m_c      out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c           (m in units of log2(e))
-// in an order that does not depend on timing.  Keys that some of an item's rows see and others do not - at most fifteen, the
+// in an order that does not depend on timing.  p is rounded to the type of V for the product with it, as in the prefix kernel, and added to l as
+// it is.  Keys that some of an item's rows see and others do not - at most fifteen, the
 // newest tokens' own - go past the tensor core: there a zero probability times whatever a later token's value holds
 // would still be NaN.
 //
